@@ -72,6 +72,46 @@ MMRS_API int mmrs_sample_token(const float *logits, int vocab, const MmrsSamplin
 MMRS_API int mmrs_token_logprob(const float *logits, int vocab, int token_id, float *out, void *workspace,
                                 size_t workspace_bytes, mmrs_stream_t stream);
 
+/* ---- verification of drafted tokens ------------------------------------------------------ */
+
+/* Sequences, logits rows and rows per sequence a call takes. */
+#define MMRS_VERIFY_MAX_SEQS 1024
+#define MMRS_VERIFY_MAX_ROWS 65536
+#define MMRS_VERIFY_MAX_Q 64
+
+/* Workspace bytes of mmrs_verify_drafts (0: arguments out of range).  Caller-owned, 256-byte
+ * aligned, zero before first use; one workspace serves one stream at a time. */
+MMRS_API size_t mmrs_verify_workspace_bytes(int num_seqs, int total_rows);
+
+/* Outcome of the last completed call on a workspace (synchronous read): MMRS_OK, or
+ * MMRS_ERR_NONFINITE when some sequence's next token could not be chosen (its place holds -1). */
+MMRS_API int mmrs_verify_workspace_status(const void *workspace);
+
+/* No counterpart in the reference (it decodes one token at a time, src/sampling.rs:84-150).
+ * Sequence b has the logits rows cu_rows[b] .. cu_rows[b + 1] - 1 of logits [total_rows][vocab]
+ * (logits_type MMRS_TYPE_F32, _F16 or _BF16 of minimax_paged.h): the target's rows after its last
+ * accepted token and after each of its d = rows - 1 drafted tokens.  Draft i of it, element
+ * cu_rows[b] - b + i of draft_tokens and uniforms and row of draft_probs [drafts][vocab] (the draft model's probabilities; null: the draft had probability 1), is judged by row i:
+ *   temperature[b] == 0: it stands when it is the row's argmax (first index of the largest);
+ *   otherwise, with p = softmax(logits / temperature[b]), when u * q(draft) < p(draft).
+ * The drafts before the first that falls are emitted, then one more token: at temperature 0 the
+ * argmax of the next row; else the argmax over the vocabulary (first index on ties) of r / noise[b],
+ * noise [num_seqs][vocab] exponential random numbers, which draws from r: p of the last row when
+ * all drafts stood, max(p - q, 0) of the row where one fell (p itself where that is nowhere
+ * positive; with draft_probs null, p without the draft).
+ * tokens int32 [num_seqs][max_q] = the emitted tokens, then -1; accepted int32 [num_seqs] = drafts
+ * that stood; logprobs f32 [num_seqs][max_q] (or null) = ln softmax(logits / T) of the emitted tokens
+ * in their rows (T = temperature, 1 where that is 0), then 0.  temperature f32 [num_seqs], or null: 1.
+ * Logits of -infinity are masked tokens.  A draft judged by a row that holds NaN or +infinity, or
+ * nothing but -infinity, falls; a next token that such a row should give is -1 (device status
+ * MMRS_ERR_NONFINITE).  Sequences without rows come last and emit nothing.  max_q bounds the rows of a
+ * sequence; total_rows bounds cu_rows. */
+MMRS_API int mmrs_verify_drafts(const void *logits, int logits_type, int vocab, const int32_t *cu_rows, int num_seqs,
+                                int total_rows, int max_q, const int32_t *draft_tokens, const float *draft_probs,
+                                const float *uniforms, const float *noise, const float *temperature, int32_t *tokens,
+                                int32_t *accepted, float *logprobs, void *workspace, size_t workspace_bytes,
+                                mmrs_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -66,6 +66,19 @@ class MmrsAttnWeights(C.Structure):
                 ("hidden", C.c_int), ("query_heads", C.c_int), ("kv_heads", C.c_int), ("rope_dim", C.c_int),
                 ("max_positions", C.c_int), ("eps", C.c_float)]
 
+
+class MmrsPagedCache(C.Structure):
+    """include/minimax_paged.h: MmrsPagedCache."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("num_pages", C.c_int), ("page_size", C.c_int), ("kv_heads", C.c_int)]
+
+
+class MmrsPagedBatch(C.Structure):
+    """include/minimax_paged.h: MmrsPagedBatch."""
+    _fields_ = [("cu_q", C.c_void_p), ("seq_len", C.c_void_p), ("page_table", C.c_void_p), ("num_seqs", C.c_int),
+                ("table_stride", C.c_int), ("total_q", C.c_int), ("max_q", C.c_int), ("max_len", C.c_int)]
+
+
 # name -> (restype, argtypes)
 PROTOTYPES = {
     "minimax_moe_decode_topk": (None, [_VP] * 7),
@@ -95,6 +108,16 @@ PROTOTYPES = {
     "mmrs_sample_workspace_status": (_I, [_VP]),
     "mmrs_sample_token": (_I, [_VP, _I, C.POINTER(MmrsSamplingParams), C.c_double, _VP, _VP, _SZ, _VP]),
     "mmrs_token_logprob": (_I, [_VP, _I, _I, _VP, _VP, _SZ, _VP]),
+    "mmrs_verify_workspace_bytes": (_SZ, [_I, _I]),
+    "mmrs_verify_workspace_status": (_I, [_VP]),
+    "mmrs_verify_drafts": (_I, [_VP, _I, _I, _VP, _I, _I, _I] + [_VP] * 9 + [_SZ, _VP]),
+    # paged 8-bit cache (include/minimax_paged.h)
+    "mmrs_paged_append": (_I, [C.POINTER(MmrsPagedCache), C.POINTER(MmrsPagedBatch), _VP, _VP, _VP, _I64, _I64, _I64,
+                               _I, _I, _VP, _VP, _I, _I, _VP, _I, _VP]),
+    "mmrs_paged_attend_workspace_bytes": (_SZ, [_I] * 4),
+    "mmrs_paged_attend_status": (_I, [_VP]),
+    "mmrs_paged_attend": (_I, [C.POINTER(MmrsPagedCache), C.POINTER(MmrsPagedBatch), _VP, _I64, _I, _I, _F, _I, _I,
+                               _VP, _VP, _VP, _SZ, _VP]),
     "mmrs_attn_decode_forward": (_I, [C.POINTER(MmrsAttnWeights), _VP, _VP, _I, _VP, _VP, _VP, _VP, _SZ, _VP]),
     "launch_tp2_peer_all_reduce_f32": (None, [_VP] * 8 + [C.c_uint, _I, _F, _VP]),
     "launch_tp2_peer_broadcast_f32": (None, [_VP] * 4 + [C.c_uint, _I, _I, _VP]),
@@ -395,3 +418,203 @@ def rmsnorm(x, weight, y=None, eps: float = 1e-6, stream=None):
     check(lib().mmrs_rmsnorm_f32(x.data_ptr(), weight.data_ptr(), y.data_ptr(), n, x.numel() // n, eps,
                                  _stream(stream)), "mmrs_rmsnorm_f32")
     return y
+
+
+# ---------------------------------------------------------------------------------------------
+# Several sequences: a paged 8-bit cache, attention over it, drafted tokens
+# ---------------------------------------------------------------------------------------------
+HEAD_DIM = 128  # MMRS_PAGED_HEAD_DIM
+PAGE_SIZES = (16, 32, 64, 128)
+
+
+def _type_code(dtype) -> int:
+    import torch
+    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}.get(dtype)
+    if code is None:
+        raise MoeError(MMRS_ERR_UNSUPPORTED, f"element type {dtype}")
+    return code
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise MoeError(MMRS_ERR_ARG, what)
+
+
+def _token_stride(t, heads: int, what: str) -> int:
+    """Elements between the token rows of t [tokens][heads][128], whose rows are contiguous."""
+    if t.shape[0] == 0:
+        return heads * HEAD_DIM
+    _need(t.dim() == 3 and t.shape[1] == heads and t.shape[2] == HEAD_DIM and t.stride(2) == 1 and
+          (heads == 1 or t.stride(1) == HEAD_DIM), f"{what}: [tokens][{heads}][{HEAD_DIM}], heads side by side")
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), heads * HEAD_DIM)
+
+
+class PagedBatch:
+    """The sequences of one call (MmrsPagedBatch): cu_q int32 [n + 1], seq_len int32 [n] (with the call's
+    new tokens) and page_table int32 [n][pages], on the device; max_q and max_len bound the numbers of
+    new tokens and the lengths, so that neither is read back."""
+
+    def __init__(self, cu_q, seq_len, page_table, max_q: int, max_len: int, total_q: int | None = None):
+        import torch
+        n = seq_len.numel()
+        for t, name in ((cu_q, "cu_q"), (seq_len, "seq_len"), (page_table, "page_table")):
+            _need(t.dtype == torch.int32 and t.is_cuda, f"{name}: int32 on the device")
+        _need(cu_q.numel() == n + 1 and cu_q.is_contiguous() and seq_len.is_contiguous(), "cu_q [n + 1], seq_len [n]")
+        _need(page_table.dim() == 2 and page_table.shape[0] == n and (page_table.stride(1) == 1 or n == 0),
+              "page_table [n][pages]")
+        self.t = (cu_q, seq_len, page_table)
+        self.num_seqs, self.total_q = n, total_q
+        # a row stride larger than the row is only ever indexed up to max_len
+        self.c = MmrsPagedBatch(cu_q.data_ptr(), seq_len.data_ptr(), page_table.data_ptr(), n,
+                                page_table.stride(0) if n > 1 else page_table.shape[1], total_q or 0, max_q, max_len)
+        self._pages = page_table.shape[1]
+        self.max_len = max_len
+
+    def bind(self, cache: "PagedKvCache", tokens: int):
+        """The C struct for a call with `tokens` token rows."""
+        _need(self._pages * cache.page_size >= self.max_len or self.num_seqs == 0, "page_table: too few pages for max_len")
+        _need(self.total_q is None or self.total_q == tokens, "total_q")
+        self.c.total_q = tokens
+        return C.byref(self.c)
+
+
+class PagedKvCache:
+    """One layer's keys and values for several sequences, in pages of 16 to 128 positions: e4m3 codes
+    [pages][kv_heads][page_size][128] and one f32 scale per page and head (a code's value is code x
+    scale).  `append` writes a batch's new tokens, `attend` is the attention of those tokens."""
+
+    def __init__(self, num_pages: int, device, kv_heads: int = 8, page_size: int = 64):
+        import torch
+        shape = (num_pages, kv_heads, page_size, HEAD_DIM)
+        self._bind(*(torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn) for _ in range(2)),
+                   *(torch.zeros(shape[:2], dtype=torch.float32, device=device) for _ in range(2)))
+
+    @classmethod
+    def from_tensors(cls, k, v, k_scale, v_scale) -> "PagedKvCache":
+        """A cache over the caller's own tensors."""
+        self = cls.__new__(cls)
+        self._bind(k, v, k_scale, v_scale)
+        return self
+
+    def _bind(self, k, v, k_scale, v_scale):
+        import torch
+        _need(k.dim() == 4 and k.shape == v.shape and k.shape[3] == HEAD_DIM and k.dtype == v.dtype ==
+              torch.float8_e4m3fn and k.is_contiguous() and v.is_contiguous(),
+              "k, v: contiguous float8_e4m3fn [pages][kv_heads][page_size][128]")
+        _need(k_scale.shape == v_scale.shape == k.shape[:2] and k_scale.dtype == v_scale.dtype == torch.float32 and
+              k_scale.is_contiguous() and v_scale.is_contiguous(), "k_scale, v_scale: f32 [pages][kv_heads]")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        pages, self.kv_heads, self.page_size = k.shape[:3]
+        if self.page_size not in PAGE_SIZES:
+            raise MoeError(MMRS_ERR_UNSUPPORTED, f"page_size {self.page_size}")
+        self.c = MmrsPagedCache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages,
+                                self.page_size, self.kv_heads)
+        self.ws = None
+
+    def append(self, batch: PagedBatch, q, k, v, rope_cos, rope_sin, q_out=None, stream=None):
+        """Writes the rotated k and v [tokens][kv_heads][128] (f32, f16 or bf16; row slices of one wider
+        tensor will do) at the batch's positions; returns the rotated q (bf16 for bf16 queries, else
+        f16; None for q None).  rope_cos / rope_sin: f32 [positions][rope_dim / 2]."""
+        import torch
+        n = k.shape[0]
+        _need(v.shape[0] == n and (q is None or q.shape[0] == n), "q, k, v: the same tokens")
+        code = _type_code(k.dtype)
+        _need(v.dtype == k.dtype and (q is None or q.dtype == k.dtype), "q, k, v: one element type")
+        _need(rope_cos.dtype == rope_sin.dtype == torch.float32 and rope_cos.shape == rope_sin.shape and
+              rope_cos.is_contiguous() and rope_sin.is_contiguous(), "rope_cos, rope_sin: f32 [positions][rope_dim / 2]")
+        heads = q_stride = out_code = 0
+        if q is not None:
+            heads = q.shape[1]
+            q_stride = _token_stride(q, heads, "q")
+            if q_out is None:
+                q_out = torch.empty(n, heads, HEAD_DIM, device=q.device,
+                                    dtype=torch.bfloat16 if code == 2 else torch.float16)
+            _need(q_out.shape == q.shape and q_out.is_contiguous(), "q_out: contiguous, shaped as q")
+            out_code = _type_code(q_out.dtype)
+        rc = lib().mmrs_paged_append(C.byref(self.c), batch.bind(self, n), _ptr(q), k.data_ptr(), v.data_ptr(), q_stride,
+                                     _token_stride(k, self.kv_heads, "k"), _token_stride(v, self.kv_heads, "v"), code,
+                                     heads, rope_cos.data_ptr(), rope_sin.data_ptr(), 2 * rope_cos.shape[1],
+                                     rope_cos.shape[0], _ptr(q_out), out_code, _stream(stream))
+        check(rc, "mmrs_paged_append")
+        return q_out
+
+    def workspace(self, num_seqs: int, tokens: int, query_heads: int):
+        import torch
+        need = lib().mmrs_paged_attend_workspace_bytes(num_seqs, tokens, query_heads, self.kv_heads)
+        if need == 0:
+            raise MoeError(MMRS_ERR_UNSUPPORTED, "mmrs_paged_attend_workspace_bytes")
+        if self.ws is None or self.ws.numel() < need:
+            self.ws = torch.zeros(need, dtype=torch.uint8, device=self.k.device)
+        return self.ws
+
+    def status(self) -> int:
+        """MMRS_OK, or MMRS_ERR_TIMEOUT when a bounded wait in an attention kernel expired (synchronous)."""
+        return MMRS_OK if self.ws is None else lib().mmrs_paged_attend_status(self.ws.data_ptr())
+
+    def attend(self, batch: PagedBatch, q, scale: float | None = None, window: int = 0, sinks: int = 0, out=None,
+               lse=None, stream=None):
+        """out [tokens][heads][128] = attention of q (f16 or bf16, rotated) over the batch's positions up to
+        each token's own; with window > 0 only the last `window` of them and the first `sinks`.  lse
+        f32 [tokens][heads] is filled when given.  scale: 1 / sqrt(128) unless given.  The calls of
+        one cache share a workspace: keep them on one stream."""
+        import torch
+        n, heads = q.shape[0], q.shape[1]
+        stride = _token_stride(q, heads, "q")
+        if out is None:
+            out = torch.empty(n, heads, HEAD_DIM, dtype=q.dtype, device=q.device)
+        _need(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous(), "out: contiguous, shaped as q")
+        _need(lse is None or (lse.dtype == torch.float32 and lse.shape == q.shape[:2] and lse.is_contiguous()),
+              "lse: f32 [tokens][heads]")
+        ws = self.workspace(batch.num_seqs, n, heads)
+        rc = lib().mmrs_paged_attend(C.byref(self.c), batch.bind(self, n), q.data_ptr(), stride, _type_code(q.dtype),
+                                     heads, HEAD_DIM ** -0.5 if scale is None else scale, window, sinks, out.data_ptr(),
+                                     _ptr(lse), ws.data_ptr(), ws.numel(), _stream(stream))
+        check(rc, "mmrs_paged_attend")
+        return out
+
+
+class DraftVerifier:
+    """Verification of drafted tokens (mmrs_verify_drafts) with this object's outputs and workspace, for up
+    to max_seqs sequences of max_q logits rows (drafts + 1) and max_rows rows in all."""
+
+    def __init__(self, vocab: int, device, max_seqs: int, max_rows: int, max_q: int):
+        import torch
+        need = lib().mmrs_verify_workspace_bytes(max_seqs, max_rows)
+        if need == 0 or max_seqs < 1:
+            raise MoeError(MMRS_ERR_ARG, "mmrs_verify_workspace_bytes")
+        self.vocab, self.max_seqs, self.max_rows, self.max_q = vocab, max_seqs, max_rows, max_q
+        self.ws = torch.zeros(need, dtype=torch.uint8, device=device)
+        self.tokens = torch.full((max_seqs, max_q), -1, dtype=torch.int32, device=device)
+        self.accepted = torch.zeros(max_seqs, dtype=torch.int32, device=device)
+        self.logprobs = torch.zeros(max_seqs, max_q, dtype=torch.float32, device=device)
+
+    def status(self) -> int:
+        """MMRS_OK, or MMRS_ERR_NONFINITE when some next token of the last call is -1 (synchronous)."""
+        return lib().mmrs_verify_workspace_status(self.ws.data_ptr())
+
+    def verify(self, logits, cu_rows, draft_tokens, uniforms, noise, draft_probs=None, temperature=None, stream=None):
+        """(tokens [n][max_q] int32, accepted [n] int32, logprobs [n][max_q] f32), valid until the next call:
+        the drafts that stand and one more token a sequence, -1 (0.0) after them.  logits [rows][vocab]
+        (f32, f16, bf16), cu_rows int32 [n + 1], draft_tokens int32 and uniforms f32 [drafts],
+        draft_probs f32 [drafts][vocab] or None (drafts that were certain), noise f32 [n][vocab]
+        (exponential), temperature f32 [n] or None (1)."""
+        import torch
+        n, rows = cu_rows.numel() - 1, logits.shape[0]
+        _need(0 <= n <= self.max_seqs and rows <= self.max_rows, "more sequences or rows than the verifier was made for")
+        _need(logits.dim() == 2 and logits.shape[1] == self.vocab and logits.is_contiguous(), "logits [rows][vocab]")
+        _need(cu_rows.dtype == torch.int32 and draft_tokens.dtype == torch.int32, "cu_rows, draft_tokens: int32")
+        _need(uniforms.dtype == torch.float32 and uniforms.numel() == draft_tokens.numel() >= rows - n, "uniforms [drafts]")
+        _need(noise.dtype == torch.float32 and noise.shape == (n, self.vocab) and noise.is_contiguous(),
+              "noise f32 [n][vocab]")
+        _need(draft_probs is None or (draft_probs.dtype == torch.float32 and draft_probs.is_contiguous() and
+                                      draft_probs.shape == (draft_tokens.numel(), self.vocab)),
+              "draft_probs f32 [drafts][vocab]")
+        _need(temperature is None or (temperature.dtype == torch.float32 and temperature.numel() == n),
+              "temperature f32 [n]")
+        rc = lib().mmrs_verify_drafts(logits.data_ptr(), _type_code(logits.dtype), self.vocab, cu_rows.data_ptr(), n, rows,
+                                      self.max_q, draft_tokens.data_ptr(), _ptr(draft_probs), uniforms.data_ptr(),
+                                      noise.data_ptr(), _ptr(temperature), self.tokens.data_ptr(),
+                                      self.accepted.data_ptr(), self.logprobs.data_ptr(), self.ws.data_ptr(),
+                                      self.ws.numel(), _stream(stream))
+        check(rc, "mmrs_verify_drafts")
+        return self.tokens[:n], self.accepted[:n], self.logprobs[:n]
