@@ -3,9 +3,10 @@
 // One CTA takes 16 rows (new tokens times the query heads of one KV head) of a sequence and walks
 // the sequence's positions in tiles of 32 with the running maximum and sum of a softmax.
 #include <cuda_runtime.h>
-#include <math.h>
 
-#include "paged.cuh"
+#include <mutex>
+
+#include "paged_attend.cuh"
 
 namespace mmrs {
 namespace {
@@ -13,17 +14,6 @@ namespace {
 constexpr int kPaThreads = 128;
 constexpr int kPaRows = 16;
 constexpr int kPaKeys = 32;
-
-struct PaParams {
-    MmrsPagedCache c;
-    MmrsPagedBatch b;
-    const void *q;
-    void *out;
-    float *lse;
-    long q_stride;
-    int query_heads, group, window, sinks;
-    float scale;
-};
 
 template <typename T>
 __global__ void __launch_bounds__(kPaThreads) paged_attend_simple_kernel(const __grid_constant__ PaParams p) {
@@ -74,7 +64,7 @@ __global__ void __launch_bounds__(kPaThreads) paged_attend_simple_kernel(const _
             if (sees) {
                 x = 0.0f;
                 for (int d = 0; d < kPgDim; ++d) x = fmaf(s_q[r][d], s_k[key][d], x);
-                x *= p.scale;
+                x *= p.scale_log2 * kPaLn2;
             }
             s_p[r][key] = x;
         }
@@ -113,20 +103,55 @@ __global__ void __launch_bounds__(kPaThreads) paged_attend_simple_kernel(const _
     }
 }
 
-size_t pa_workspace_bytes(int num_seqs, int total_q, int query_heads, int kv_heads) {
-    if (num_seqs < 0 || num_seqs > MMRS_PAGED_MAX_SEQS || total_q < 0 || kv_heads < 1 || query_heads < kv_heads ||
-        query_heads % kv_heads || query_heads / kv_heads > MMRS_PAGED_MAX_GROUP)
-        return 0;
-    return 256;
+// Workspace: a status word, one counter per (sequence, KV head), two partial results per CTA.
+constexpr size_t kPaSlot = sizeof(float) * 32 * (kPgDim + 2);
+struct PaLayout {
+    size_t counters, partials, total;
+};
+PaLayout pa_layout(int num_seqs, int kv_heads) {
+    PaLayout l;
+    l.counters = 256;
+    l.partials = l.counters + (sizeof(uint32_t) * num_seqs * kv_heads + 255) / 256 * 256;
+    l.total = l.partials + kPaSlot * 2 * pa_sm_count();
+    return l;
 }
 
 }  // namespace
+
+int pa_sm_count() {
+    static std::once_flag once[64];
+    static int sms[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    std::call_once(once[dev], [dev] {
+        int n = 0;
+        sms[dev] = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && n > 0 ? n : 148;
+    });
+    return sms[dev];
+}
+
+int pa_make_map(CUtensorMap *map, const void *codes, const MmrsPagedCache &c, int rows) {
+    const auto encode = tensor_map_encoder();
+    if (!encode) return MMRS_ERR_LAUNCH;
+    const cuuint64_t dims[2] = {(cuuint64_t)kPgDim, (cuuint64_t)c.num_pages * c.kv_heads * c.page_size};
+    const cuuint64_t strides[1] = {(cuuint64_t)kPgDim};
+    const cuuint32_t box[2] = {(cuuint32_t)kPgDim, (cuuint32_t)rows}, elem[2] = {1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(codes), dims, strides, box, elem,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? MMRS_OK
+               : MMRS_ERR_LAUNCH;
+}
+
 }  // namespace mmrs
 
 using namespace mmrs;
 
 extern "C" size_t mmrs_paged_attend_workspace_bytes(int num_seqs, int total_q, int query_heads, int kv_heads) {
-    return pa_workspace_bytes(num_seqs, total_q, query_heads, kv_heads);
+    if (num_seqs < 0 || num_seqs > kPaMaxSeqs || total_q < 0 || kv_heads < 1 || query_heads < kv_heads ||
+        query_heads % kv_heads || query_heads / kv_heads > MMRS_PAGED_MAX_GROUP)
+        return 0;
+    return pa_layout(num_seqs, kv_heads).total;
 }
 
 extern "C" int mmrs_paged_attend_status(const void *workspace) {
@@ -150,7 +175,7 @@ extern "C" int mmrs_paged_attend(const MmrsPagedCache *cache, const MmrsPagedBat
         q_stride < (int64_t)query_heads * kPgDim)
         return MMRS_ERR_ARG;
     if (!workspace || ((uintptr_t)workspace & 255u) ||
-        workspace_bytes < pa_workspace_bytes(batch->num_seqs, batch->total_q, query_heads, cache->kv_heads))
+        workspace_bytes < pa_layout(batch->num_seqs, cache->kv_heads).total)
         return MMRS_ERR_ARG;
     PaParams p = {};
     p.c = *cache;
@@ -159,7 +184,20 @@ extern "C" int mmrs_paged_attend(const MmrsPagedCache *cache, const MmrsPagedBat
     p.q_stride = q_stride;
     p.query_heads = query_heads, p.group = query_heads / cache->kv_heads;
     p.window = window, p.sinks = sinks;
-    p.scale = scale;
+    p.scale_log2 = scale * kPaLog2e;
+    const PaLayout l = pa_layout(batch->num_seqs, cache->kv_heads);
+    uint8_t *ws = static_cast<uint8_t *>(workspace);
+    p.status = reinterpret_cast<uint32_t *>(ws);
+    p.counters = reinterpret_cast<uint32_t *>(ws + l.counters);
+    p.partials = reinterpret_cast<float *>(ws + l.partials);
+    // units of work (16 positions of a KV head) are counted with 32 bits
+    if ((long)batch->num_seqs * cache->kv_heads * ((batch->max_len + 15) / 16) > 0x3fffffffL) return MMRS_ERR_UNSUPPORTED;
+    if ((long)batch->max_q * p.group <= 32) {
+        CUtensorMap kmap, vmap;
+        int mc = pa_make_map(&kmap, cache->k, *cache, 16);
+        if (mc == MMRS_OK) mc = pa_make_map(&vmap, cache->v, *cache, 16);
+        return mc != MMRS_OK ? mc : pa_launch_decode(p, kmap, vmap, type, (cudaStream_t)stream);
+    }
     const long tiles = ((long)batch->max_q * p.group + kPaRows - 1) / kPaRows;
     if (tiles > 0x7fffffffL || cache->kv_heads > 65535) return MMRS_ERR_UNSUPPORTED;
     const dim3 grid((unsigned)tiles, cache->kv_heads, batch->num_seqs);

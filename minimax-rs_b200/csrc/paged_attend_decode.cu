@@ -1,0 +1,543 @@
+// Paged attention for few rows: single tokens and drafted tokens (at most 32 rows a KV head).
+//
+// Each K / V code is read once and used for all rows of its KV head, so the kernel is bound by HBM:
+// 256 bytes a position and head.  The products run on mma.sync with the operands turned round, S^T =
+// K Q^T and O^T += V^T P^T: the 16 positions of a step are the 16 rows of an instruction and eight
+// query rows its columns, so that six query heads waste two columns of eight instead of ten rows
+// of sixteen.  Which code goes to which contraction index is free as long as both operands agree,
+// so a lane takes 32 consecutive codes of a key row (two 16-byte reads) and 16 of a value row, and
+// turns them into f16 pairs in registers (e4m3 to f16 is exact).  P^T comes from S^T's accumulators
+// by a transposing move of 8x8 tiles.
+//
+// Work: the steps of 16 positions of all sequences and KV heads form one list, of which every CTA
+// (one per SM) takes an equal, contiguous part; a CTA's eight warps take its steps in turn, each
+// with a ring of TMA copies of its own, its own running maximum and sum, and no barrier until the end
+// of a (sequence, head).  Where that end lies in another CTA, the CTAs' partial results go through
+// the workspace and the last to arrive joins them in order.
+#include "paged_attend.cuh"
+
+#include <algorithm>
+#include <mutex>
+
+namespace mmrs {
+namespace {
+
+constexpr int kPdWarps = 8;
+constexpr int kPdThreads = 32 * kPdWarps;
+constexpr int kPdStep = 16;                       // positions of a step
+constexpr int kPdTile = kPdStep * kPgDim;         // bytes of its keys (or values)
+constexpr int kPdStages = 5;
+constexpr int kPdRowFloats = kPgDim + 4;          // a row of the merge buffer
+
+struct PdShared {
+    uint8_t ring[kPdWarps][kPdStages][2][kPdTile];  // 1024-byte aligned tiles (swizzled)
+    float o[kPdWarps][8][kPdRowFloats];             // one eight-row group of every warp's sums
+    uint32_t q[8][4][32][2];                        // NT = 3, 4: the queries' fragments
+    float m[kPdWarps][32], l[kPdWarps][32];
+    float meta[kPdWarps][kPdStages][2];             // scales of the stage's page (k < 0: nothing there)
+    uint64_t full[kPdWarps][kPdStages];
+    int prefix[kPaMaxSeqs + 1];
+    int scan[kPdWarps];
+    int last;
+};
+
+__device__ __forceinline__ void pd_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pd_transpose(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ uint4 pd_lds(const uint8_t *tile, int row, int chunk) {
+    return *reinterpret_cast<const uint4 *>(tile + row * kPgDim + ((chunk ^ (row & 7)) << 4));
+}
+// Four codes -> two f16 pairs.
+__device__ __forceinline__ void pd_cvt(uint32_t x, uint32_t &lo, uint32_t &hi) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(x));
+}
+
+// An item's piece in this CTA's part of the list: sequence b, KV head h, steps [off, off + n) of the
+// item's nb.
+struct PdSeg {
+    int b, h, off, n, nb;
+    PgSeq seq;
+    PaSpan<kPdStep> span;
+};
+
+template <int NT, typename T>
+struct PdKernel {
+    static constexpr int kRows = 8 * NT;
+    static constexpr bool kQShared = NT > 2;
+
+    static __device__ int item_steps(const PaParams &p, int b, PgSeq &seq, PaSpan<kPdStep> &span) {
+        seq = pg_seq(p.b, p.c.page_size, b);
+        span = pa_span<kPdStep>(max(seq.pos0, 0), seq.len - 1, p.window, p.sinks);
+        return seq.count > 0 ? max(span.n, 1) : 0;  // rows that see nothing are written too
+    }
+
+    // The piece that starts at unit u (< end, the CTA's end; `total` units in all).
+    static __device__ void seek(const PaParams &p, const PdShared &sm, int u, int end, PdSeg &s) {
+        int lo = 0, hi = p.b.num_seqs;  // the last sequence with prefix <= u
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (sm.prefix[mid] <= u) lo = mid;
+            else hi = mid;
+        }
+        s.b = lo;
+        s.nb = item_steps(p, lo, s.seq, s.span);
+        const int at = u - sm.prefix[lo];
+        s.h = at / s.nb;
+        s.off = at - s.h * s.nb;
+        s.n = min(s.nb - s.off, end - u);
+    }
+
+    static __device__ void load_q(const PaParams &p, const PdSeg &s, int lane, int nt, uint32_t (&f)[16], float &factor) {
+        const int r = nt * 8 + (lane >> 2), t = lane & 3;
+        factor = 1.0f;
+        if (r >= s.seq.count * p.group) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) f[i] = 0u;
+            return;
+        }
+        const T *q = static_cast<const T *>(p.q) + (long)(s.seq.row0 + r / p.group) * p.q_stride +
+                     (s.h * p.group + r % p.group) * kPgDim + 32 * t;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint4 v = reinterpret_cast<const uint4 *>(q)[i];
+            f[4 * i] = v.x, f[4 * i + 1] = v.y, f[4 * i + 2] = v.z, f[4 * i + 3] = v.w;
+        }
+    }
+    // bf16 queries become f16 with the row's largest value moved to [2^14, 2^15): exact but for
+    // values 2^-38 of it and less.  Returns what the products have to be multiplied by.
+    static __device__ float to_f16(uint32_t (&f)[16]) {
+        if constexpr (sizeof(T) == 2 && !__is_same(T, __half)) {
+            float amax = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(f[i] << 16)), fabsf(__uint_as_float(f[i] & 0xffff0000u))));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+            const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127 - 14, -120), 120);
+            const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                f[i] = pg_pack2(__uint_as_float(f[i] << 16) * down, __uint_as_float(f[i] & 0xffff0000u) * down,
+                                (const __half *)nullptr);
+            return up;
+        }
+        return 1.0f;
+    }
+
+    static __device__ void write_row(const PaParams &p, const PdSeg &s, int r, int lane, float4 o, float m, float l) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const long at = (long)(s.seq.row0 + r / p.group) * p.query_heads + s.h * p.group + r % p.group;
+        T *out = static_cast<T *>(p.out) + at * kPgDim;
+        reinterpret_cast<uint2 *>(out)[lane] =
+            make_uint2(pg_pack2(o.x * inv, o.y * inv, out), pg_pack2(o.z * inv, o.w * inv, out));
+        if (p.lse && lane == 0) p.lse[at] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kPaLn2;
+    }
+
+    static __device__ void run(const PaParams &p, const CUtensorMap *kmap, const CUtensorMap *vmap, PdShared &sm) {
+        const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+        const uint64_t deadline = globaltimer_ns() + kPaTimeoutNs;
+        if (lane == 0) {
+            for (int i = 0; i < kPdStages; ++i) mbar_init(&sm.full[warp][i], 1);
+            fence_mbar_init();
+        }
+        // prefix sums of the sequences' units: each thread takes four consecutive sequences
+        int mine[kPaMaxSeqs / kPdThreads], sum = 0;
+#pragma unroll
+        for (int i = 0; i < kPaMaxSeqs / kPdThreads; ++i) {
+            const int b = tid * (kPaMaxSeqs / kPdThreads) + i;
+            PgSeq seq;
+            PaSpan<kPdStep> span;
+            mine[i] = b < p.b.num_seqs ? item_steps(p, b, seq, span) * p.c.kv_heads : 0;
+            sum += mine[i];
+        }
+        int incl = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += up;
+        }
+        if (lane == 31) sm.scan[warp] = incl;
+        __syncthreads();
+        int before = incl - sum, total = 0;
+#pragma unroll
+        for (int w = 0; w < kPdWarps; ++w) {
+            if (w < warp) before += sm.scan[w];
+            total += sm.scan[w];
+        }
+#pragma unroll
+        for (int i = 0; i < kPaMaxSeqs / kPdThreads; ++i) {
+            sm.prefix[tid * (kPaMaxSeqs / kPdThreads) + i] = before;
+            before += mine[i];
+        }
+        __syncthreads();
+        const int share = max((total + (int)gridDim.x - 1) / (int)gridDim.x, kPdWarps);
+        const int u0 = min((long)share * blockIdx.x, (long)total), u1 = min(u0 + share, total);
+        if (u0 >= u1) return;
+
+        // ---- the copies: a cursor over this warp's steps, up to kPdStages ahead of the products
+        PdSeg in;
+        int in_u = u0, in_i = warp, in_base = 0, issued = 0;
+        int pid = -1;
+        float ks = 0.0f, vs = 0.0f;
+        bool in_open = false, in_done = false;
+        auto issue = [&]() {
+            while (!in_done) {
+                if (!in_open) {
+                    seek(p, sm, in_u, u1, in);
+                    in_i = warp;
+                    in_base = -1;
+                    in_open = true;
+                }
+                if (in_i < in.n) break;
+                in_u += in.n;
+                in_open = false;
+                in_done = in_u >= u1;
+            }
+            if (in_done) return;
+            const int batch = (in_i - warp) / (32 * kPdWarps);
+            if (batch != in_base) {  // the pages and scales of this warp's next 32 steps, one a lane
+                in_base = batch;
+                const int i = warp + kPdWarps * (batch * 32 + lane);
+                pid = -1;
+                if (i < in.n) {
+                    const int j = in.span.step(in.off + i) * kPdStep;
+                    if (j < in.seq.len) pid = p.b.page_table[(long)in.b * p.b.table_stride + j / p.c.page_size];
+                    if (pid >= p.c.num_pages) pid = -1;
+                }
+                if (pid >= 0) {
+                    ks = p.c.k_scale[(long)pid * p.c.kv_heads + in.h];
+                    vs = p.c.v_scale[(long)pid * p.c.kv_heads + in.h];
+                }
+            }
+            const int src = (in_i - warp) / kPdWarps & 31;
+            const int page = __shfl_sync(0xffffffffu, pid, src);
+            const float k1 = __shfl_sync(0xffffffffu, ks, src), v1 = __shfl_sync(0xffffffffu, vs, src);
+            if (lane == 0) {
+                const int st = issued % kPdStages;
+                sm.meta[warp][st][0] = page < 0 ? -1.0f : k1;
+                sm.meta[warp][st][1] = v1;
+                if (page < 0) {
+                    mbar_arrive(&sm.full[warp][st]);
+                } else {
+                    const int j = in.span.step(in.off + in_i) * kPdStep;
+                    const int row = (page * p.c.kv_heads + in.h) * p.c.page_size + j % p.c.page_size;
+                    mbar_arrive_expect_tx(&sm.full[warp][st], 2 * kPdTile);
+                    pa_tma_2d(sm.ring[warp][st][0], kmap, 0, row, &sm.full[warp][st]);
+                    pa_tma_2d(sm.ring[warp][st][1], vmap, 0, row, &sm.full[warp][st]);
+                }
+            }
+            ++issued;
+            in_i += kPdWarps;
+        };
+        for (int i = 0; i < kPdStages; ++i) issue();
+
+        bool failed = false;
+        int used = 0;
+        for (int u = u0; u < u1;) {
+            PdSeg s;
+            seek(p, sm, u, u1, s);
+            const int rows = min(s.seq.count * p.group, kRows);
+            uint32_t qf[kQShared ? 1 : NT][16];
+            float qs[NT][2];  // the score's factor for this lane's two columns
+            int pos[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float up = 1.0f;
+                if (!kQShared || warp == nt) {
+                    uint32_t f[16];
+                    load_q(p, s, lane, nt, f, up);
+                    up = to_f16(f);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        if constexpr (kQShared) sm.q[i / 2][nt][lane][i & 1] = f[i];
+                        else qf[nt][i] = f[i];
+                    }
+                    if constexpr (kQShared)
+                        if (t == 0) sm.m[0][nt * 8 + g] = up;
+                }
+                if constexpr (!kQShared) {
+                    qs[nt][0] = __shfl_sync(0xffffffffu, up, 8 * t) * p.scale_log2;
+                    qs[nt][1] = __shfl_sync(0xffffffffu, up, 8 * t + 4) * p.scale_log2;
+                }
+            }
+            if constexpr (kQShared) {
+                __syncthreads();
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) qs[nt][c] = sm.m[0][nt * 8 + 2 * t + c] * p.scale_log2;
+                __syncthreads();
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int r = nt * 8 + 2 * t + c;
+                    pos[nt][c] = r < rows ? s.seq.pos0 + r / p.group : -1;
+                }
+            const int pos_lo = s.seq.pos0, pos_hi = s.seq.len - 1;
+            float m[NT][2], l[NT][2], o[NT][8][4];
+            float vref = 0.0f;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) m[nt][c] = -INFINITY, l[nt][c] = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) o[nt][j][c] = 0.0f;
+            }
+            for (int i = warp; i < s.n; i += kPdWarps, ++used) {
+                const int st = used % kPdStages;
+                if (!failed && !mbar_wait_bounded(&sm.full[warp][st], (used / kPdStages) & 1, deadline)) {
+                    failed = true;
+                    atomicExch(p.status, (uint32_t)MMRS_ERR_TIMEOUT);
+                }
+                __syncwarp();
+                const float ksc = sm.meta[warp][st][0], vsc = sm.meta[warp][st][1];
+                if (ksc >= 0.0f || ksc != ksc) {
+                    const int j0 = s.span.step(s.off + i) * kPdStep;
+                    const uint8_t *kt = sm.ring[warp][st][0], *vt = sm.ring[warp][st][1];
+                    float sc[NT][4];
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) sc[nt][c] = 0.0f;
+                    {
+                        uint32_t k0[8], k1[8];
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const uint4 x = pd_lds(kt, g, 2 * t + c), y = pd_lds(kt, g + 8, 2 * t + c);
+                            k0[4 * c] = x.x, k0[4 * c + 1] = x.y, k0[4 * c + 2] = x.z, k0[4 * c + 3] = x.w;
+                            k1[4 * c] = y.x, k1[4 * c + 1] = y.y, k1[4 * c + 2] = y.z, k1[4 * c + 3] = y.w;
+                        }
+#pragma unroll
+                        for (int ks8 = 0; ks8 < 8; ++ks8) {
+                            uint32_t a0, a1, a2, a3;
+                            pd_cvt(k0[ks8], a0, a2);
+                            pd_cvt(k1[ks8], a1, a3);
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                if constexpr (kQShared) {
+                                    const uint2 b = *reinterpret_cast<const uint2 *>(sm.q[ks8][nt][lane]);
+                                    pd_mma(sc[nt], a0, a1, a2, a3, b.x, b.y);
+                                } else {
+                                    pd_mma(sc[nt], a0, a1, a2, a3, qf[nt][2 * ks8], qf[nt][2 * ks8 + 1]);
+                                }
+                            }
+                        }
+                    }
+                    const bool whole = j0 + kPdStep - 1 <= pos_lo &&
+                                       (p.window <= 0 || pos_hi - j0 < p.window || j0 + kPdStep <= p.sinks);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            sc[nt][c] *= qs[nt][c & 1] * ksc;
+                            if (!whole && !pa_sees(j0 + g + (c >> 1) * 8, pos[nt][c & 1], p.window, p.sinks))
+                                sc[nt][c] = -INFINITY;
+                        }
+                    // the values' scale: probabilities are stored relative to the largest seen
+                    float vfac = 1.0f;
+                    if (vsc > vref) {
+                        vfac = vref / vsc;
+                        vref = vsc;
+                    }
+                    const float vr = vref > 0.0f ? vsc / vref : 0.0f;
+                    uint32_t pb[NT][2];
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float p4[4];
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            float mx = fmaxf(sc[nt][c], sc[nt][c + 2]);
+                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                            mx = fmaxf(mx, m[nt][c]);
+                            const float base = mx == -INFINITY ? 0.0f : mx;
+                            const float fac = pa_exp2(m[nt][c] - base);
+                            m[nt][c] = mx;
+                            p4[c] = pa_exp2(sc[nt][c] - base);
+                            p4[c + 2] = pa_exp2(sc[nt][c + 2] - base);
+                            l[nt][c] = l[nt][c] * fac + p4[c] + p4[c + 2];
+                            const float of = fac * vfac;
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) o[nt][j][c] *= of, o[nt][j][c + 2] *= of;
+                        }
+                        pb[nt][0] = pd_transpose(pg_pack2(p4[0] * vr, p4[1] * vr, (const __half *)nullptr));
+                        pb[nt][1] = pd_transpose(pg_pack2(p4[2] * vr, p4[3] * vr, (const __half *)nullptr));
+                    }
+                    uint4 v4[4];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const int row = 2 * t + (c & 1) + (c >> 1) * 8;
+                        v4[c] = pd_lds(vt, row, g);
+                        // slots past the sequence's end may hold anything
+                        if (!whole && j0 + row >= s.seq.len) v4[c] = make_uint4(0u, 0u, 0u, 0u);
+                    }
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const uint32_t x[4] = {reinterpret_cast<const uint32_t *>(&v4[0])[w],
+                                               reinterpret_cast<const uint32_t *>(&v4[1])[w],
+                                               reinterpret_cast<const uint32_t *>(&v4[2])[w],
+                                               reinterpret_cast<const uint32_t *>(&v4[3])[w]};
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            const uint32_t sel = half ? 0x7362u : 0x5140u;
+                            uint32_t a0, a1, a2, a3;
+                            pd_cvt(__byte_perm(x[0], x[1], sel), a0, a1);
+                            pd_cvt(__byte_perm(x[2], x[3], sel), a2, a3);
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+                                pd_mma(o[nt][2 * w + half], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+                        }
+                    }
+                }
+                __syncwarp();
+                issue();
+            }
+            // ---- the eight warps' results of this piece
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], x);
+                    if (g == 0) sm.m[warp][nt * 8 + 2 * t + c] = m[nt][c], sm.l[warp][nt * 8 + 2 * t + c] = l[nt][c];
+                }
+            const int end = u - s.off + s.nb;  // the unit after the item
+            const int c0 = (u - s.off) / share, c1 = (end - 1) / share;
+            float *slot = p.partials + ((size_t)blockIdx.x * 2 + ((int)blockIdx.x == c0 ? 1 : 0)) * (32 * (kPgDim + 2));
+            __syncthreads();
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int r = nt * 8 + 2 * t + c;
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int w = 0; w < kPdWarps; ++w) top = fmaxf(top, sm.m[w][r]);
+                    const float f = top == -INFINITY ? 1.0f : pa_exp2(m[nt][c] - top);
+#pragma unroll
+                    for (int j = 0; j < 8; j += 2)
+                        *reinterpret_cast<float4 *>(&sm.o[warp][2 * t + c][16 * g + 2 * j]) =
+                            make_float4(o[nt][j][c] * f * vref, o[nt][j][c + 2] * f * vref, o[nt][j + 1][c] * f * vref,
+                                        o[nt][j + 1][c + 2] * f * vref);
+                }
+                __syncthreads();
+                {
+                    const int r = nt * 8 + warp;  // eight warps, eight rows
+                    float top = -INFINITY, sum_l = 0.0f;
+#pragma unroll
+                    for (int w = 0; w < kPdWarps; ++w) top = fmaxf(top, sm.m[w][r]);
+                    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                    for (int w = 0; w < kPdWarps; ++w) {
+                        sum_l += sm.l[w][r] * (top == -INFINITY ? 1.0f : pa_exp2(sm.m[w][r] - top));
+                        const float4 x = *reinterpret_cast<const float4 *>(&sm.o[w][warp][4 * lane]);
+                        acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
+                    }
+                    if (r < rows) {
+                        if (c0 == c1) {
+                            write_row(p, s, r, lane, acc, top, sum_l);
+                        } else {
+                            reinterpret_cast<float4 *>(slot + r * kPgDim)[lane] = acc;
+                            if (lane == 0) slot[32 * kPgDim + r] = top, slot[32 * kPgDim + 32 + r] = sum_l;
+                        }
+                    }
+                }
+                __syncthreads();
+            }
+            if (c0 != c1) {
+                uint32_t *counter = p.counters + (s.b * p.c.kv_heads + s.h);
+                if (tid == 0) {
+                    __threadfence();
+                    sm.last = atomicAdd(counter, 1u) == (uint32_t)(c1 - c0);
+                    __threadfence();
+                }
+                __syncthreads();
+                if (sm.last) {
+                    for (int r = warp; r < rows; r += kPdWarps) {
+                        float top = -INFINITY, sum_l = 0.0f;
+                        auto at = [&](int c) {
+                            return p.partials + ((size_t)c * 2 + (c == c0 ? 1 : 0)) * (32 * (kPgDim + 2));
+                        };
+                        for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, __ldcg(at(c) + 32 * kPgDim + r));
+                        top = warp_max_butterfly(top);
+                        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+                        for (int c = c0; c <= c1; ++c) {
+                            const float *a = at(c);
+                            const float f = top == -INFINITY ? 1.0f : pa_exp2(__ldcg(a + 32 * kPgDim + r) - top);
+                            const float4 x = __ldcg(reinterpret_cast<const float4 *>(a + r * kPgDim) + lane);
+                            sum_l += f * __ldcg(a + 32 * kPgDim + 32 + r);
+                            acc.x += f * x.x, acc.y += f * x.y, acc.z += f * x.z, acc.w += f * x.w;
+                        }
+                        write_row(p, s, r, lane, acc, top, sum_l);
+                    }
+                    if (tid == 0) *counter = 0u;
+                }
+            }
+            u += s.n;
+        }
+        if (failed)  // copies that came late must not land in another block's memory
+            for (int i = used < kPdStages ? 0 : used - kPdStages; i < issued; ++i)
+                mbar_wait_bounded(&sm.full[warp][i % kPdStages], (i / kPdStages) & 1, deadline + kPaTimeoutNs);
+    }
+};
+
+template <int NT, typename T>
+__global__ void __launch_bounds__(kPdThreads, 1)
+    paged_attend_decode_kernel(const __grid_constant__ PaParams p, const __grid_constant__ CUtensorMap kmap,
+                               const __grid_constant__ CUtensorMap vmap) {
+    extern __shared__ uint8_t raw[];
+    PdShared &sm = *reinterpret_cast<PdShared *>(raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u));
+    PdKernel<NT, T>::run(p, &kmap, &vmap, sm);
+}
+
+constexpr size_t kPdSmem = sizeof(PdShared) + 1024;
+static_assert(kPdSmem <= 227 * 1024, "shared memory");
+
+template <int NT, typename T>
+int pd_launch(const PaParams &p, const CUtensorMap &k, const CUtensorMap &v, cudaStream_t s) {
+    static std::once_flag once[64];
+    static cudaError_t set_rc[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return MMRS_ERR_LAUNCH;
+    std::call_once(once[dev], [dev] {
+        set_rc[dev] = cudaFuncSetAttribute(paged_attend_decode_kernel<NT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           (int)kPdSmem);
+    });
+    if (set_rc[dev] != cudaSuccess) return MMRS_ERR_LAUNCH;
+    paged_attend_decode_kernel<NT, T><<<pa_sm_count(), kPdThreads, kPdSmem, s>>>(p, k, v);
+    return cudaGetLastError() == cudaSuccess ? MMRS_OK : MMRS_ERR_LAUNCH;
+}
+
+template <typename T>
+int pd_launch_rows(const PaParams &p, const CUtensorMap &k, const CUtensorMap &v, cudaStream_t s) {
+    const int rows = p.b.max_q * p.group;
+    if (rows <= 8) return pd_launch<1, T>(p, k, v, s);
+    if (rows <= 16) return pd_launch<2, T>(p, k, v, s);
+    if (rows <= 24) return pd_launch<3, T>(p, k, v, s);
+    return pd_launch<4, T>(p, k, v, s);
+}
+
+}  // namespace
+
+int pa_launch_decode(const PaParams &p, const CUtensorMap &k, const CUtensorMap &v, int type, cudaStream_t s) {
+    return type == MMRS_TYPE_F16 ? pd_launch_rows<__half>(p, k, v, s) : pd_launch_rows<__nv_bfloat16>(p, k, v, s);
+}
+
+}  // namespace mmrs
