@@ -10,6 +10,7 @@
 namespace mmrs {
 
 constexpr int kPaMaxSeqs = MMRS_PAGED_MAX_SEQS;
+constexpr int kPaDecodeRows = 32;  // rows of a KV head up to which the decode kernel runs
 constexpr float kPaLog2e = 1.4426950408889634f;
 constexpr float kPaLn2 = 0.6931471805599453f;
 constexpr uint64_t kPaTimeoutNs = 2000000000ull;
@@ -24,8 +25,8 @@ struct PaParams {
     int query_heads, group, window, sinks;
     float scale_log2;     // scale * log2(e)
     uint32_t *status;     // workspace: status word
-    uint32_t *counters;   // workspace: one per item that several CTAs share, zero between calls
-    float *partials;      // workspace: two slots per CTA
+    uint32_t *counters;   // workspace: one per CTA (for the item it begins and others end), zero between calls
+    float *partials;      // workspace: two slots per CTA, for the items it shares with CTAs before and after it
 };
 
 // The positions that some new token of a sequence sees, in steps of kStep: the steps [0, ns) of
@@ -76,5 +77,6 @@ int pa_sm_count();
 
 // Kernels' launchers.
 int pa_launch_decode(const PaParams &p, const CUtensorMap &k, const CUtensorMap &v, int type, cudaStream_t s);
+int pa_launch_prompt(const PaParams &p, int type, cudaStream_t s);
 
 }  // namespace mmrs

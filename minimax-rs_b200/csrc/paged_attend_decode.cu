@@ -461,7 +461,7 @@ struct PdKernel {
                 __syncthreads();
             }
             if (c0 != c1) {
-                uint32_t *counter = p.counters + (s.b * p.c.kv_heads + s.h);
+                uint32_t *counter = p.counters + c0;
                 if (tid == 0) {
                     __threadfence();
                     sm.last = atomicAdd(counter, 1u) == (uint32_t)(c1 - c0);

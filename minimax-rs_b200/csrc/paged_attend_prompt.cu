@@ -1,0 +1,692 @@
+// Paged attention of many rows: prompt chunks, and drafts of more than 32 rows a KV head.
+//
+// Here every code is used by hundreds of rows, so the kernel is bound by arithmetic: 4 * 128 flops
+// a (row, position) on the tensor cores and one exponential, and the two weigh about the same on
+// an SM (a 128x128 tile takes 1024 cycles of either).  The rows of a KV head (new tokens x query
+// heads of its group) are packed 256 to an item, two M = 128 tiles whose softmax and products
+// alternate, so that one tile's exponentials run under the other's products:
+//   warps 0-3, 4-7   softmax of tile 0, 1, one thread a row: S from tensor memory, running maximum
+//                    and sum, P (f16) back into S's columns, and the epilogue
+//   warps 8-11       K and V codes from global memory through registers (one tile ahead), e4m3 to
+//                    f16 (exact), into the operand layouts
+//   warp 12          issues S = Q K^T (both operands in shared memory) and O += P V (P in tensor
+//                    memory), kind::f16
+// Operand tiles are without swizzle: 16-byte pieces (8 columns of one row) with the eight rows of a
+// core matrix next to each other; the same form serves K (K-major) and V (its columns are the
+// product's N, so the tile is read MN-major).
+//
+// Scales: a page's key scale multiplies its columns' scores in the exponent's FMA; its value scale,
+// relative to the largest of the piece, is added there as a logarithm, so neither costs a product
+// per element.  The running maximum moves only when it grows by more than 2^8 (P stays below f16's
+// range), which leaves O alone on almost every tile.
+//
+// Work: the (item, 128-position tile) pairs of all sequences form one list, of which each CTA (one
+// per SM) takes an equal contiguous part; an item cut by that gets its pieces joined through the
+// workspace by the CTA that finishes last, in order.
+#include "paged_attend.cuh"
+#include "umma.cuh"
+
+#include <mutex>
+
+namespace mmrs {
+namespace {
+
+constexpr int kPpThreads = 13 * 32;
+constexpr int kPpKeys = 128;                 // positions of a tile
+constexpr int kPpRows = 256;                 // rows of an item
+constexpr int kPpTile = 128 * kPgDim * 2;    // bytes of an operand tile
+constexpr int kPpSlice = 128 * 16;           // bytes between 8-column slices of a tile
+constexpr int kPpStages = 2;
+constexpr int kPpScales = 4;                 // tiles whose scales are kept
+constexpr float kPpLazy = 8.0f;              // log2 of how far P may exceed 1
+constexpr float kPpMinRel = -60.0f;          // log2 of the smallest value scale told from 0
+constexpr int kPpConvWarp0 = 8, kPpMmaWarp = 12;
+
+struct PpScale {  // of the eight 16-position groups of a tile
+    float k[8];   // key scale; < 0: the group's page holds nothing
+    float rel[8], inv[8];  // log2 of the value scale over vref, and vref over the value scale
+    float vref;
+};
+struct PpShared {
+    uint8_t q[2][kPpTile], k[kPpStages][kPpTile], v[kPpStages][kPpTile];
+    PpScale sc[kPpScales];
+    float vmax[4];
+    int prefix[kPaMaxSeqs + 1];
+    uint64_t q_full[2], s_full[2], p_full[2], o_done[2];
+    uint64_t k_full[kPpStages], k_empty[kPpStages], v_full[kPpStages], v_empty[kPpStages], sc_full[kPpScales];
+    uint64_t mdone;
+    uint32_t tmem;
+    int abort, last;
+};
+constexpr size_t kPpSmem = sizeof(PpShared) + 128;
+static_assert(kPpSmem <= 227 * 1024, "shared memory");
+
+constexpr uint32_t kPpIdesc = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);  // f16 x f16 -> f32, 128 x 128
+constexpr uint32_t kPpIdescV = kPpIdesc | (1u << 16);                                 // B read MN-major
+constexpr uint32_t kColS = 0, kColO = 256;
+
+__device__ __forceinline__ void pp_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void pp_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void pp_ld32(uint32_t taddr, float (&v)[32]) {
+    uint32_t *u = reinterpret_cast<uint32_t *>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
+        "%30,%31}, [%32];"
+        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+          "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]),
+          "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]),
+          "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void pp_st16(uint32_t taddr, const uint32_t (&u)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(
+            u[0]),
+        "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]), "r"(u[10]),
+        "r"(u[11]), "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(taddr)
+        : "memory");
+}
+// Waits for the loads; `v` passes through so that no use of it moves before the wait.
+__device__ __forceinline__ void pp_wait_ld(float (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]),
+                   "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])
+                 :
+                 : "memory");
+    asm volatile(""
+                 : "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]),
+                   "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void pp_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Bounded wait of one role: false when two seconds have passed or another role has given up.
+__device__ __forceinline__ bool pp_wait(uint64_t *bar, uint32_t parity, PpShared &sm, const PaParams &p) {
+    if (mbar_test_wait(bar, parity)) return true;
+    uint64_t start = 0;
+    uint32_t spins = 0;
+    while (!mbar_try_wait(bar, parity)) {
+        if ((++spins & 255u)) continue;
+        if (*reinterpret_cast<volatile int *>(&sm.abort)) return false;
+        const uint64_t now = globaltimer_ns();
+        if (start == 0) start = now;
+        if (now - start > kPaTimeoutNs) {
+            *reinterpret_cast<volatile int *>(&sm.abort) = 1;
+            atomicExch(p.status, (uint32_t)MMRS_ERR_TIMEOUT);
+            return false;
+        }
+    }
+    return true;
+}
+
+// The same for a whole warp, with one answer.
+__device__ __forceinline__ bool pp_wait_warp(uint64_t *bar, uint32_t parity, PpShared &sm, const PaParams &p) {
+    return __all_sync(0xffffffffu, pp_wait(bar, parity, sm, p)) != 0;
+}
+
+// An item's piece: sequence b, KV head h, rows [row0, row0 + rows) of the sequence's packed rows,
+// tiles [off, off + n) of the item's nb.
+struct PpSeg {
+    int b, h, row0, rows, off, n, nb;
+    PgSeq seq;
+    PaSpan<kPpKeys> span;
+};
+
+__device__ __forceinline__ int pp_tiles(const PaParams &p, const PgSeq &seq, int rt, PaSpan<kPpKeys> &span) {
+    const int total = seq.count * p.group, last = min((rt + 1) * kPpRows, total) - 1;
+    const int lo = max(seq.pos0 + rt * kPpRows / p.group, 0), hi = seq.pos0 + last / p.group;
+    span = pa_span<kPpKeys>(lo, max(hi, -1), p.window, p.sinks);
+    return max(span.n, 1);  // rows that see nothing are written too
+}
+// Units of one KV head of a sequence (whole warp).
+__device__ int pp_seq_units(const PaParams &p, const PgSeq &seq, int lane) {
+    const int tiles = (seq.count * p.group + kPpRows - 1) / kPpRows;
+    int sum = 0;
+    PaSpan<kPpKeys> span;
+    for (int rt = lane; rt < tiles; rt += 32) sum += pp_tiles(p, seq, rt, span);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return sum;
+}
+// The piece that starts at unit u (whole warp).
+__device__ void pp_seek(const PaParams &p, const PpShared &sm, int u, int end, int lane, PpSeg &s) {
+    int lo = 0, hi = p.b.num_seqs;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (sm.prefix[mid] <= u) lo = mid;
+        else hi = mid;
+    }
+    s.b = lo;
+    s.seq = pg_seq(p.b, p.c.page_size, lo);
+    const int per_head = (sm.prefix[lo + 1] - sm.prefix[lo]) / p.c.kv_heads;
+    int at = u - sm.prefix[lo];
+    s.h = at / per_head;
+    at -= s.h * per_head;
+    const int tiles = (s.seq.count * p.group + kPpRows - 1) / kPpRows;
+    int rt = 0, before = 0;
+    for (int r0 = 0; r0 < tiles; r0 += 32) {
+        PaSpan<kPpKeys> span;
+        const int n = r0 + lane < tiles ? pp_tiles(p, s.seq, r0 + lane, span) : 0;
+        int incl = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += up;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, before + incl > at);
+        if (past) {
+            const int l = __ffs(past) - 1;
+            rt = r0 + l;
+            s.off = at - before - __shfl_sync(0xffffffffu, incl - n, l);
+            break;
+        }
+        before += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    s.nb = pp_tiles(p, s.seq, rt, s.span);
+    s.n = min(s.nb - s.off, end - u);
+    s.row0 = rt * kPpRows;
+    s.rows = min(kPpRows, s.seq.count * p.group - s.row0);
+}
+
+// ---- warps 8-11: codes to f16 operand tiles ------------------------------------------------------
+// Thread: key (lane & 7) of each of its warp's four 8-key groups, 16-code chunks (lane >> 3) and + 4.
+__device__ __forceinline__ void pp_store_tile(uint8_t *tile, const uint4 (&raw)[8], int w, int lane) {
+#pragma unroll
+    for (int it = 0; it < 8; ++it) {
+        const int group = w * 4 + (it >> 1), chunk = (it & 1) * 4 + (lane >> 3);
+        uint8_t *at = tile + 2 * chunk * kPpSlice + group * 128 + (lane & 7) * 16;
+        const uint4 r = raw[it];
+        uint4 a, b;
+        a.x = pg_e4m3x2_to_half2(r.x & 0xffffu), a.y = pg_e4m3x2_to_half2(r.x >> 16);
+        a.z = pg_e4m3x2_to_half2(r.y & 0xffffu), a.w = pg_e4m3x2_to_half2(r.y >> 16);
+        b.x = pg_e4m3x2_to_half2(r.z & 0xffffu), b.y = pg_e4m3x2_to_half2(r.z >> 16);
+        b.z = pg_e4m3x2_to_half2(r.w & 0xffffu), b.w = pg_e4m3x2_to_half2(r.w >> 16);
+        *reinterpret_cast<uint4 *>(at) = a;
+        *reinterpret_cast<uint4 *>(at + kPpSlice) = b;
+    }
+}
+
+__device__ void pp_convert(const PaParams &p, PpShared &sm, int u0, int u1) {
+    const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) - kPpConvWarp0;
+    int tile = 0;
+    bool ok = true;  // after a failed wait only the barriers among these warps go on
+    for (int u = u0; u < u1;) {
+        PpSeg s;
+        pp_seek(p, sm, u, u1, lane, s);
+        const int ps = p.c.page_size;
+        // the pages and scales of this warp's two 16-position groups in 16 tiles, one a lane
+        int pid = -1;
+        float ks = 0.0f, vs = 0.0f;
+        auto fetch = [&](int base) {
+            const int i = base + (lane >> 1);
+            pid = -1, ks = -1.0f, vs = 0.0f;
+            if (i < s.n) {
+                const int j = s.span.step(s.off + i) * kPpKeys + w * 32 + (lane & 1) * 16;
+                if (j < s.seq.len) pid = p.b.page_table[(long)s.b * p.b.table_stride + j / ps];
+                if (pid >= p.c.num_pages) pid = -1;
+                if (pid >= 0) {
+                    ks = p.c.k_scale[(long)pid * p.c.kv_heads + s.h];
+                    vs = p.c.v_scale[(long)pid * p.c.kv_heads + s.h];
+                }
+            }
+        };
+        float vref = 0.0f;
+        for (int base = 0; base < s.n; base += 16) {
+            fetch(base);
+            vref = fmaxf(vref, vs);
+        }
+        vref = warp_max_butterfly(vref);
+        named_sync(2, 128);
+        if (lane == 0) sm.vmax[w] = vref;
+        named_sync(2, 128);
+        vref = fmaxf(fmaxf(sm.vmax[0], sm.vmax[1]), fmaxf(sm.vmax[2], sm.vmax[3]));
+        if (!(vref > 0.0f)) vref = 1.0f;
+        uint4 kr[8], vr[8];
+        auto load = [&](const void *codes, int i, uint4 (&r)[8]) {
+            const int key0 = s.span.step(s.off + i) * kPpKeys + w * 32 + (lane & 7);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int page = __shfl_sync(0xffffffffu, pid, (i & 15) * 2 + half);
+#pragma unroll
+                for (int it = half * 4; it < half * 4 + 4; ++it) {
+                    const int key = key0 + (it >> 1) * 8, chunk = (it & 1) * 4 + (lane >> 3);
+                    r[it] = make_uint4(0u, 0u, 0u, 0u);
+                    // slots past the sequence's end may hold anything
+                    if (page >= 0 && key < s.seq.len)
+                        r[it] = __ldg(reinterpret_cast<const uint4 *>(
+                                          static_cast<const uint8_t *>(codes) +
+                                          (((long)page * p.c.kv_heads + s.h) * ps + (key & (ps - 1))) * kPgDim) +
+                                      chunk);
+                }
+            }
+        };
+        fetch(0);
+        load(p.c.k, 0, kr);
+        load(p.c.v, 0, vr);
+        for (int i = 0; ok && i < s.n; ++i, ++tile) {
+            const int st = tile % kPpStages, use = tile / kPpStages;
+            PpScale &sc = sm.sc[tile % kPpScales];
+            if ((lane >> 1) == (i & 15)) {
+                const int g = 2 * w + (lane & 1);
+                const float rel = fmaxf(log2f(vs / vref), kPpMinRel);
+                sc.k[g] = ks, sc.rel[g] = rel, sc.inv[g] = exp2f(-rel);
+            }
+            if (w == 0 && lane == 0) sc.vref = vref;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.sc_full[tile % kPpScales]);
+            if (!(ok = pp_wait_warp(&sm.k_empty[st], (use & 1) ^ 1, sm, p))) break;
+            pp_store_tile(sm.k[st], kr, w, lane);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.k_full[st]);
+            if (i + 1 < s.n) {
+                if (((i + 1) & 15) == 0) fetch(i + 1);
+                load(p.c.k, i + 1, kr);
+            }
+            if (!(ok = pp_wait_warp(&sm.v_empty[st], (use & 1) ^ 1, sm, p))) break;
+            pp_store_tile(sm.v[st], vr, w, lane);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.v_full[st]);
+            if (i + 1 < s.n) load(p.c.v, i + 1, vr);
+        }
+        u += s.n;
+    }
+}
+
+// ---- warp 12: the products -----------------------------------------------------------------------
+__device__ void pp_products(const PaParams &p, PpShared &sm, int u0, int u1) {
+    const int lane = threadIdx.x & 31;
+    const uint32_t tmem = sm.tmem;
+    int tile = 0, pieces[2] = {0, 0}, used[2] = {0, 0};  // tiles so far; pieces, tiles of each row tile
+    // K-major operands: 16-byte K slices kPpSlice apart, 8-row groups 128 apart; V (MN-major): 8-key
+    // groups 128 apart, 8-column groups kPpSlice apart
+    auto scores = [&](int i, int st) {
+        const uint64_t a = umma_smem_desc(smem_u32(sm.q[i]), kPpSlice, 128);
+        const uint64_t b = umma_smem_desc(smem_u32(sm.k[st]), kPpSlice, 128);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            pp_mma_ss(tmem + kColS + 128 * i, a + (uint64_t)(k * 2 * kPpSlice >> 4), b + (uint64_t)(k * 2 * kPpSlice >> 4),
+                      kPpIdesc, k > 0);
+        tc_commit(&sm.s_full[i]);
+    };
+    auto values = [&](int i, int st, bool first) {
+        const uint64_t b = umma_smem_desc(smem_u32(sm.v[st]), 128, kPpSlice);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            pp_mma_ts(tmem + kColO + 128 * i, tmem + kColS + 128 * i + 8 * k, b + (uint64_t)(k * 256 >> 4), kPpIdescV,
+                      !(first && k == 0));
+        tc_commit(&sm.o_done[i]);
+    };
+    bool ok = true;
+    for (int u = u0; ok && u < u1;) {
+        PpSeg s;
+        pp_seek(p, sm, u, u1, lane, s);
+        const int tiles = s.rows > 128 ? 2 : 1;
+        if (lane == 0) {
+            auto wait = [&](uint64_t *bar, int use) {
+                ok = ok && pp_wait(bar, (uint32_t)use & 1, sm, p);
+                tc_fence_after();
+                return ok;
+            };
+            wait(&sm.k_full[tile % kPpStages], tile / kPpStages);
+            for (int i = 0; i < tiles; ++i)
+                if (wait(&sm.q_full[i], pieces[i])) scores(i, tile % kPpStages);
+            if (ok) tc_commit(&sm.k_empty[tile % kPpStages]);
+            for (int j = 0; ok && j < s.n; ++j) {
+                const int at = tile + j, st = at % kPpStages, next = (at + 1) % kPpStages;
+                wait(&sm.v_full[st], at / kPpStages);
+                for (int i = 0; i < tiles; ++i) {
+                    if (!wait(&sm.p_full[i], used[i] + j)) break;
+                    values(i, st, j == 0);
+                    if (i == tiles - 1) tc_commit(&sm.v_empty[st]);
+                    if (j + 1 == s.n) continue;
+                    // the products end in the order of their issue: P is read before S's next tile
+                    // overwrites it
+                    if (i == 0 && !wait(&sm.k_full[next], (at + 1) / kPpStages)) break;
+                    scores(i, next);
+                    if (i == tiles - 1) tc_commit(&sm.k_empty[next]);
+                }
+            }
+        }
+        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+        tile += s.n;
+        for (int i = 0; i < tiles; ++i) ++pieces[i], used[i] += s.n;
+        u += s.n;
+    }
+    if (lane == 0) {  // every product has ended before the tensor memory goes
+        tc_commit(&sm.mdone);
+        mbar_wait_bounded(&sm.mdone, 0, globaltimer_ns() + kPaTimeoutNs);
+    }
+    __syncwarp();
+}
+
+// ---- warps 0-7: softmax and epilogue ----------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ float pp_load_q(const PaParams &p, const PpSeg &s, int r, uint8_t *tile, int row) {
+    uint4 f[16];
+    const T *q = static_cast<const T *>(p.q) + (long)(s.seq.row0 + r / p.group) * p.q_stride +
+                 (s.h * p.group + r % p.group) * kPgDim;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) f[i] = reinterpret_cast<const uint4 *>(q)[i];
+    uint32_t *w = reinterpret_cast<uint32_t *>(f);
+    float up = 1.0f;
+    if constexpr (!__is_same(T, __half)) {
+        // to f16 with the row's largest value moved to [2^14, 2^15): exact but for values 2^-38 of it
+        // and less
+        float amax = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 64; ++i)
+            amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
+        const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127 - 14, -120), 120);
+        const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+        up = __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+        for (int i = 0; i < 64; ++i)
+            w[i] = pg_pack2(__uint_as_float(w[i] << 16) * down, __uint_as_float(w[i] & 0xffff0000u) * down,
+                            (const __half *)nullptr);
+    }
+    const uint32_t sign = p.scale_log2 < 0.0f ? 0x80008000u : 0u;  // the columns' factors stay >= 0
+    uint8_t *at = tile + (row >> 3) * 128 + (row & 7) * 16;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        *reinterpret_cast<uint4 *>(at + i * kPpSlice) =
+            make_uint4(f[i].x ^ sign, f[i].y ^ sign, f[i].z ^ sign, f[i].w ^ sign);
+    return up * fabsf(p.scale_log2);
+}
+
+template <typename T>
+__device__ __forceinline__ void pp_write8(T *out, const float *o, float f) {
+    *reinterpret_cast<uint4 *>(out) =
+        make_uint4(pg_pack2(o[0] * f, o[1] * f, out), pg_pack2(o[2] * f, o[3] * f, out), pg_pack2(o[4] * f, o[5] * f, out),
+                   pg_pack2(o[6] * f, o[7] * f, out));
+}
+
+constexpr size_t kPpSlotFloats = (size_t)kPpRows * (kPgDim + 2);
+
+template <typename T>
+__device__ void pp_softmax(const PaParams &p, PpShared &sm, int u0, int u1, int share) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i = warp >> 2;
+    const int row = (warp & 3) * 32 + lane;  // row of the tile, and lane of the tensor memory
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t ts = sm.tmem + lanes + kColS + 128 * i, to = sm.tmem + lanes + kColO + 128 * i;
+    int tile = 0, used = 0;
+    bool ok = true;  // after a failed wait only the barriers among these warps go on
+    for (int u = u0; u < u1;) {
+        PpSeg s;
+        pp_seek(p, sm, u, u1, lane, s);
+        const int end = u - s.off + s.nb, c0 = (u - s.off) / share, c1 = (end - 1) / share;
+        float *slot = p.partials + ((size_t)blockIdx.x * 2 + ((int)blockIdx.x == c0 ? 1 : 0)) * kPpSlotFloats;
+        if (ok && (i == 0 || s.rows > 128)) {
+            const int r = i * 128 + row;  // of the item
+            const bool live = r < s.rows, warp_live = i * 128 + (warp & 3) * 32 < s.rows;
+            const int pos = live ? s.seq.pos0 + (s.row0 + r) / p.group : -1;
+            float m = -INFINITY, l = 0.0f, factor = 0.0f, vref = 1.0f;
+            if (live) factor = pp_load_q<T>(p, s, s.row0 + r, sm.q[i], row);
+            fence_proxy_async_smem();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.q_full[i]);
+            for (int j = 0; j < s.n; ++j) {
+                const int at = tile + j;
+                ok = pp_wait_warp(&sm.s_full[i], (uint32_t)(used + j) & 1, sm, p) &&
+                     pp_wait_warp(&sm.sc_full[at % kPpScales], (uint32_t)(at / kPpScales) & 1, sm, p);
+                if (!ok) break;
+                tc_fence_after();
+                if (warp_live) {
+                    const PpScale &sc = sm.sc[at % kPpScales];
+                    const int key0 = s.span.step(s.off + j) * kPpKeys;
+                    vref = sc.vref;
+                    bool whole = key0 + kPpKeys - 1 <= pos &&
+                                 (p.window <= 0 || pos - key0 < p.window || key0 + kPpKeys <= p.sinks);
+                    float col[8];
+#pragma unroll
+                    for (int g = 0; g < 8; ++g) {
+                        whole = whole && !(sc.k[g] < 0.0f);
+                        col[g] = sc.k[g] * factor;
+                    }
+                    whole = __all_sync(0xffffffffu, whole);
+                    auto sees = [&](int g, int x) {
+                        return !(sc.k[g] < 0.0f) && pa_sees(key0 + g * 16 + x, pos, p.window, p.sinks);
+                    };
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        float v[32];
+                        pp_ld32(ts + 32 * c, v);
+                        pp_wait_ld(v);
+#pragma unroll
+                        for (int g = 0; g < 2; ++g) {
+                            float mx = -INFINITY;
+                            if (whole) {
+#pragma unroll
+                                for (int x = 0; x < 16; ++x) mx = fmaxf(mx, v[16 * g + x]);
+                            } else {
+#pragma unroll
+                                for (int x = 0; x < 16; ++x) mx = sees(2 * c + g, x) ? fmaxf(mx, v[16 * g + x]) : mx;
+                            }
+                            if (mx != -INFINITY) top = fmaxf(top, mx * col[2 * c + g]);
+                        }
+                    }
+                    const bool grows = top > m + kPpLazy || (m == -INFINITY && top != -INFINITY);
+                    if (j == 0) {
+                        m = top;
+                    } else if (__any_sync(0xffffffffu, grows)) {
+                        const float now = fmaxf(m, top), f = now == -INFINITY ? 1.0f : pa_exp2(m - now);
+                        m = now;
+                        l *= f;
+                        if (!(ok = pp_wait_warp(&sm.o_done[i], (uint32_t)(used + j - 1) & 1, sm, p))) break;
+                        tc_fence_after();
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            float v[32];
+                            pp_ld32(to + 32 * c, v);
+                            pp_wait_ld(v);
+                            uint32_t w[2][16];
+#pragma unroll
+                            for (int x = 0; x < 32; ++x) w[x >> 4][x & 15] = __float_as_uint(v[x] * f);
+                            pp_st16(to + 32 * c, w[0]);
+                            pp_st16(to + 32 * c + 16, w[1]);
+                        }
+                        pp_wait_st();
+                    }
+                    const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        float v[32];
+                        pp_ld32(ts + 32 * c, v);
+                        pp_wait_ld(v);
+                        uint32_t w[16];
+#pragma unroll
+                        for (int g = 0; g < 2; ++g) {
+                            const float add = sc.rel[2 * c + g] - base;
+                            float sum = 0.0f;
+#pragma unroll
+                            for (int x = 0; x < 16; x += 2) {
+                                float e0 = pa_exp2(fmaf(v[16 * g + x], col[2 * c + g], add));
+                                float e1 = pa_exp2(fmaf(v[16 * g + x + 1], col[2 * c + g], add));
+                                if (!whole) {
+                                    e0 = sees(2 * c + g, x) ? e0 : 0.0f;
+                                    e1 = sees(2 * c + g, x + 1) ? e1 : 0.0f;
+                                }
+                                sum += e0 + e1;
+                                w[8 * g + x / 2] = pg_pack2(e0, e1, (const __half *)nullptr);
+                            }
+                            l += sum * sc.inv[2 * c + g];
+                        }
+                        pp_st16(ts + 16 * c, w);  // these columns of S have been read
+                    }
+                    pp_wait_st();
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.p_full[i]);
+            }
+            ok = ok && pp_wait_warp(&sm.o_done[i], (uint32_t)(used + s.n - 1) & 1, sm, p);
+            tc_fence_after();
+            used += s.n;
+            if (ok && warp_live) {
+                const long dst = (long)(s.seq.row0 + (s.row0 + r) / p.group) * p.query_heads + s.h * p.group +
+                                 (s.row0 + r) % p.group;
+                const float f = c0 != c1 ? vref : l == 0.0f ? 0.0f : vref / l;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float v[32];
+                    pp_ld32(to + 32 * c, v);
+                    pp_wait_ld(v);
+                    if (live && c0 == c1) {
+                        T *out = static_cast<T *>(p.out) + dst * kPgDim + 32 * c;
+#pragma unroll
+                        for (int x = 0; x < 32; x += 8) pp_write8(out + x, v + x, f);
+                    } else if (live) {
+                        float4 *out = reinterpret_cast<float4 *>(slot + (size_t)r * kPgDim + 32 * c);
+#pragma unroll
+                        for (int x = 0; x < 8; ++x)
+                            out[x] = make_float4(v[4 * x] * f, v[4 * x + 1] * f, v[4 * x + 2] * f, v[4 * x + 3] * f);
+                    }
+                }
+                if (live && c0 == c1) {
+                    if (p.lse) p.lse[dst] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kPaLn2;
+                } else if (live) {
+                    slot[(size_t)kPpRows * kPgDim + r] = m;
+                    slot[(size_t)kPpRows * (kPgDim + 1) + r] = l;
+                }
+            }
+            tc_fence_before();
+        }
+        if (c0 != c1) {
+            named_sync(1, 256);
+            if (threadIdx.x == 0) {
+                __threadfence();
+                sm.last = !sm.abort && atomicAdd(p.counters + c0, 1u) == (uint32_t)(c1 - c0);
+                __threadfence();
+            }
+            named_sync(1, 256);
+            if (sm.last) {
+                for (int r = warp; r < s.rows; r += 8) {
+                    auto at = [&](int c) { return p.partials + ((size_t)c * 2 + (c == c0 ? 1 : 0)) * kPpSlotFloats; };
+                    float top = -INFINITY, l = 0.0f;
+                    for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, __ldcg(at(c) + (size_t)kPpRows * kPgDim + r));
+                    top = warp_max_butterfly(top);
+                    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+                    for (int c = c0; c <= c1; ++c) {
+                        const float *a = at(c);
+                        const float f = top == -INFINITY ? 1.0f : pa_exp2(__ldcg(a + (size_t)kPpRows * kPgDim + r) - top);
+                        const float4 x = __ldcg(reinterpret_cast<const float4 *>(a + (size_t)r * kPgDim) + lane);
+                        l += f * __ldcg(a + (size_t)kPpRows * (kPgDim + 1) + r);
+                        acc.x += f * x.x, acc.y += f * x.y, acc.z += f * x.z, acc.w += f * x.w;
+                    }
+                    const long dst = (long)(s.seq.row0 + (s.row0 + r) / p.group) * p.query_heads + s.h * p.group +
+                                     (s.row0 + r) % p.group;
+                    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                    T *out = static_cast<T *>(p.out) + dst * kPgDim;
+                    reinterpret_cast<uint2 *>(out)[lane] =
+                        make_uint2(pg_pack2(acc.x * inv, acc.y * inv, out), pg_pack2(acc.z * inv, acc.w * inv, out));
+                    if (p.lse && lane == 0) p.lse[dst] = l == 0.0f ? -INFINITY : (top + log2f(l)) * kPaLn2;
+                }
+                if (threadIdx.x == 0) p.counters[c0] = 0u;
+            }
+        }
+        tile += s.n;
+        u += s.n;
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kPpThreads, 1) paged_attend_prompt_kernel(const __grid_constant__ PaParams p) {
+    extern __shared__ uint8_t raw[];
+    PpShared &sm = *reinterpret_cast<PpShared *>(raw + ((128u - (smem_u32(raw) & 127u)) & 127u));
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sm.q_full[i], 4), mbar_init(&sm.p_full[i], 4);
+            mbar_init(&sm.s_full[i], 1), mbar_init(&sm.o_done[i], 1);
+        }
+        for (int i = 0; i < kPpStages; ++i) {
+            mbar_init(&sm.k_full[i], 4), mbar_init(&sm.v_full[i], 4);
+            mbar_init(&sm.k_empty[i], 1), mbar_init(&sm.v_empty[i], 1);
+        }
+        for (int i = 0; i < kPpScales; ++i) mbar_init(&sm.sc_full[i], 4);
+        mbar_init(&sm.mdone, 1);
+        sm.abort = 0;
+        fence_mbar_init();
+    }
+    for (int b = warp; b < p.b.num_seqs; b += kPpThreads / 32) {
+        const int n = pp_seq_units(p, pg_seq(p.b, p.c.page_size, b), lane) * p.c.kv_heads;
+        if (lane == 0) sm.prefix[b + 1] = n;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        int before = 0;
+        if (lane == 0) sm.prefix[0] = 0;
+        for (int b = 0; b < p.b.num_seqs; b += 32) {
+            int incl = b + lane < p.b.num_seqs ? sm.prefix[b + lane + 1] : 0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int up = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += up;
+            }
+            if (b + lane < p.b.num_seqs) sm.prefix[b + lane + 1] = before + incl;
+            before += __shfl_sync(0xffffffffu, incl, 31);
+        }
+    }
+    __syncthreads();
+    const int total = sm.prefix[p.b.num_seqs];
+    const int share = max((total + (int)gridDim.x - 1) / (int)gridDim.x, 1);
+    const int u0 = (int)min((long)share * blockIdx.x, (long)total), u1 = min(u0 + share, total);
+    if (u0 >= u1) return;
+    if (warp == kPpMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp < kPpConvWarp0) pp_softmax<T>(p, sm, u0, u1, share);
+    else if (warp < kPpMmaWarp) pp_convert(p, sm, u0, u1);
+    else pp_products(p, sm, u0, u1);
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kPpMmaWarp) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(sm.tmem), "r"(512));
+    }
+}
+
+template <typename T>
+int pp_launch(const PaParams &p, cudaStream_t s) {
+    static std::once_flag once[64];
+    static cudaError_t set_rc[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return MMRS_ERR_LAUNCH;
+    std::call_once(once[dev], [dev] {
+        set_rc[dev] = cudaFuncSetAttribute(paged_attend_prompt_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           (int)kPpSmem);
+    });
+    if (set_rc[dev] != cudaSuccess) return MMRS_ERR_LAUNCH;
+    paged_attend_prompt_kernel<T><<<pa_sm_count(), kPpThreads, kPpSmem, s>>>(p);
+    return cudaGetLastError() == cudaSuccess ? MMRS_OK : MMRS_ERR_LAUNCH;
+}
+
+}  // namespace
+
+int pa_launch_prompt(const PaParams &p, int type, cudaStream_t s) {
+    return type == MMRS_TYPE_F16 ? pp_launch<__half>(p, s) : pp_launch<__nv_bfloat16>(p, s);
+}
+
+}  // namespace mmrs
