@@ -15,9 +15,10 @@
 // core matrix next to each other; the same form serves K (K-major) and V (its columns are the
 // product's N, so the tile is read MN-major).
 //
-// Scales: a page's key scale multiplies its columns' scores in the exponent's FMA; its value scale,
-// relative to the largest of the piece, is added there as a logarithm, so neither costs a product
-// per element.  The running maximum moves only when it grows by more than 2^8 (P stays below f16's
+// Scales: a page's key scale multiplies its columns' scores in the exponent's FMA.  Its value scale,
+// relative to the largest of the piece, multiplies the values on their way to f16 (exact for the
+// powers of two that the append writes, one rounding otherwise).  Neither costs the softmax anything
+// an element.  The running maximum moves only when it grows by more than 2^8 (P stays below f16's
 // range), which leaves O alone on almost every tile.
 //
 // Work: the (item, 128-position tile) pairs of all sequences form one list, of which each CTA (one
@@ -31,7 +32,7 @@
 namespace mmrs {
 namespace {
 
-constexpr int kPpThreads = 13 * 32;
+constexpr int kPpThreads = 16 * 32;  // four warpgroups; the last has one working warp
 constexpr int kPpKeys = 128;                 // positions of a tile
 constexpr int kPpRows = 256;                 // rows of an item
 constexpr int kPpTile = 128 * kPgDim * 2;    // bytes of an operand tile
@@ -39,20 +40,18 @@ constexpr int kPpSlice = 128 * 16;           // bytes between 8-column slices of
 constexpr int kPpStages = 2;
 constexpr int kPpScales = 4;                 // tiles whose scales are kept
 constexpr float kPpLazy = 8.0f;              // log2 of how far P may exceed 1
-constexpr float kPpMinRel = -60.0f;          // log2 of the smallest value scale told from 0
 constexpr int kPpConvWarp0 = 8, kPpMmaWarp = 12;
 
-struct PpScale {  // of the eight 16-position groups of a tile
-    float k[8];   // key scale; < 0: the group's page holds nothing
-    float rel[8], inv[8];  // log2 of the value scale over vref, and vref over the value scale
-    float vref;
+struct alignas(16) PpScale {  // of the eight 16-position groups of a tile
+    float k[8];  // key scale; < 0: the group's page holds nothing
+    float vref;  // what the piece's values are relative to
 };
 struct PpShared {
     uint8_t q[2][kPpTile], k[kPpStages][kPpTile], v[kPpStages][kPpTile];
     PpScale sc[kPpScales];
     float vmax[4];
     int prefix[kPaMaxSeqs + 1];
-    uint64_t q_full[2], s_full[2], p_full[2], o_done[2];
+    uint64_t q_full[2], s_full[2], p_half[2], p_full[2], o_done[2], turn[2];
     uint64_t k_full[kPpStages], k_empty[kPpStages], v_full[kPpStages], v_empty[kPpStages], sc_full[kPpScales];
     uint64_t mdone;
     uint32_t tmem;
@@ -65,18 +64,24 @@ constexpr uint32_t kPpIdesc = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 
 constexpr uint32_t kPpIdescV = kPpIdesc | (1u << 16);                                 // B read MN-major
 constexpr uint32_t kColS = 0, kColO = 256;
 
-__device__ __forceinline__ void pp_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// Descriptors as their 32-bit halves (umma_smem_desc): only the low one moves with the address.
+__device__ __forceinline__ uint32_t pp_desc_lo(uint32_t saddr, uint32_t lbo) {
+    return (saddr >> 4) | (lbo >> 4) << 16;
+}
+constexpr uint32_t pp_desc_hi(uint32_t sbo) { return (sbo >> 4) | 1u << 14; }
+__device__ __forceinline__ void pp_mma_ss(uint32_t d, uint32_t alo, uint32_t ahi, uint32_t blo, uint32_t bhi,
+                                          uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tmov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
+        "setp.ne.b32 p, %6, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n\t}" ::"r"(d),
+        "r"(alo), "r"(ahi), "r"(blo), "r"(bhi), "r"(idesc), "r"(acc)
         : "memory");
 }
-__device__ __forceinline__ void pp_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void pp_mma_ts(uint32_t d, uint32_t a, uint32_t blo, uint32_t bhi, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tmov.b64 b, {%2, %3};\n\t"
+        "setp.ne.b32 p, %5, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(blo), "r"(bhi), "r"(idesc), "r"(acc)
         : "memory");
 }
 __device__ __forceinline__ void pp_ld32(uint32_t taddr, float (&v)[32]) {
@@ -100,27 +105,116 @@ __device__ __forceinline__ void pp_st16(uint32_t taddr, const uint32_t (&u)[16])
         : "memory");
 }
 // Waits for the loads; `v` passes through so that no use of it moves before the wait.
-__device__ __forceinline__ void pp_wait_ld(float (&v)[32]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
+__device__ __forceinline__ void pp_hold32(float *v) {
+    asm volatile(""
                  : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]),
-                   "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])
-                 :
-                 : "memory");
+                   "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]));
     asm volatile(""
                  : "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]),
-                   "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31])
-                 :
-                 : "memory");
+                   "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31]));
+}
+__device__ __forceinline__ void pp_wait_ld(float (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    pp_hold32(v);
+}
+// Two f32 in one register pair: one instruction for both.
+__device__ __forceinline__ uint64_t pp_pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void pp_split(uint64_t r, float &a, float &b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
+}
+__device__ __forceinline__ uint64_t pp_fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t pp_add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// 2^x of both halves on the FMA units: x = n + f, |f| <= 1/2, 2^f by a degree-4 polynomial (relative
+// error below 2.7e-6 in f32, the least-maximum fit of 2^f; P keeps 2^-11), times 2^n made from n's
+// bits.  The special-function units give a warp four results a cycle; one pair in four this way takes
+// 20 % off a tile's exponentials (1474 -> 1108 cycles for one warp of a scheduler, 2380 -> 1908 for
+// two), and three in eight no more.  x below -126 counts as -126, NaN stays NaN.
+__device__ __forceinline__ uint64_t pp_exp2_fma(uint64_t x) {
+    float a, b;
+    pp_split(x, a, b);
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-126.0f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-126.0f));
+    x = pp_pair(a, b);
+    const uint64_t r = pp_add2(x, pp_pair(12582912.0f, 12582912.0f));  // 1.5 * 2^23: rounds to whole numbers
+    const uint64_t f = pp_fma2(pp_add2(r, pp_pair(-12582912.0f, -12582912.0f)), pp_pair(-1.0f, -1.0f), x);
+    uint64_t y = pp_fma2(f, pp_pair(0.009570102f, 0.009570102f), pp_pair(0.05591786f, 0.05591786f));
+    y = pp_fma2(y, f, pp_pair(0.24024744f, 0.24024744f));
+    y = pp_fma2(y, f, pp_pair(0.6931218f, 0.6931218f));
+    y = pp_fma2(y, f, pp_pair(0.9999993f, 0.9999993f));
+    pp_split(r, a, b);
+    a = __int_as_float((__float_as_int(a) << 23) + 0x3f800000), b = __int_as_float((__float_as_int(b) << 23) + 0x3f800000);
+    uint64_t z;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(z) : "l"(y), "l"(pp_pair(a, b)));
+    return z;
 }
 __device__ __forceinline__ void pp_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// A row of S with -infinity where the row does not see the column: x > at, with a window (at - x >=
+// window and x >= first), or a group whose page holds nothing.  A pass of its own, so that the loops
+// over S stay short enough for the instruction cache (masks unrolled there cost more than they do).
+__device__ __forceinline__ void pp_mask(uint32_t ts, int at, int window, int first, const float *ks) {
+    const int gone = window > 0 ? at - window : -1, seen = window > 0 ? first : 0;
+#pragma unroll 1
+    for (int c = 0; c < 4; ++c) {
+        float v[32];
+        pp_ld32(ts + 32 * c, v);
+        const bool none0 = ks[2 * c] < 0.0f, none1 = ks[2 * c + 1] < 0.0f;
+        pp_wait_ld(v);
+        uint32_t w[2][16];
+#pragma unroll
+        for (int x = 0; x < 32; ++x) {
+            const int y = 32 * c + x;
+            const bool hide = y > at || (y <= gone && y >= seen) || (x < 16 ? none0 : none1);
+            w[x >> 4][x & 15] = __float_as_uint(hide ? -INFINITY : v[x]);
+        }
+        pp_st16(ts + 32 * c, w[0]);
+        pp_st16(ts + 32 * c + 16, w[1]);
+    }
+    pp_wait_st();
+}
+
+// A row of O times f.
+__device__ __forceinline__ void pp_scale_o(uint32_t to, float f) {
+#pragma unroll 1
+    for (int c = 0; c < 4; ++c) {
+        float v[32];
+        pp_ld32(to + 32 * c, v);
+        pp_wait_ld(v);
+        uint32_t w[2][16];
+#pragma unroll
+        for (int x = 0; x < 32; ++x) w[x >> 4][x & 15] = __float_as_uint(v[x] * f);
+        pp_st16(to + 32 * c, w[0]);
+        pp_st16(to + 32 * c + 16, w[1]);
+    }
+    pp_wait_st();
+}
 
 // Bounded wait of one role: false when two seconds have passed or another role has given up.
 __device__ __forceinline__ bool pp_wait(uint64_t *bar, uint32_t parity, PpShared &sm, const PaParams &p) {
     if (mbar_test_wait(bar, parity)) return true;
+    // the warp sleeps in hardware until the phase ends: a spinning one takes the path that the
+    // exponentials and shared memory need
     uint64_t start = 0;
-    uint32_t spins = 0;
-    while (!mbar_try_wait(bar, parity)) {
-        if ((++spins & 255u)) continue;
+    for (;;) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)
+            : "memory");
+        if (ok) return true;
         if (*reinterpret_cast<volatile int *>(&sm.abort)) return false;
         const uint64_t now = globaltimer_ns();
         if (start == 0) start = now;
@@ -130,7 +224,6 @@ __device__ __forceinline__ bool pp_wait(uint64_t *bar, uint32_t parity, PpShared
             return false;
         }
     }
-    return true;
 }
 
 // The same for a whole warp, with one answer.
@@ -202,9 +295,19 @@ __device__ void pp_seek(const PaParams &p, const PpShared &sm, int u, int end, i
     s.rows = min(kPpRows, s.seq.count * p.group - s.row0);
 }
 
+// A read that leaves the L1 alone.
+__device__ __forceinline__ uint4 pp_ldg(const uint8_t *at) {
+    uint4 r;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+                 : "l"(at));
+    return r;
+}
+
 // ---- warps 8-11: codes to f16 operand tiles ------------------------------------------------------
 // Thread: key (lane & 7) of each of its warp's four 8-key groups, 16-code chunks (lane >> 3) and + 4.
-__device__ __forceinline__ void pp_store_tile(uint8_t *tile, const uint4 (&raw)[8], int w, int lane) {
+template <bool kScaled>
+__device__ __forceinline__ void pp_store_tile(uint8_t *tile, const uint4 (&raw)[8], int w, int lane, const __half2 *rel) {
 #pragma unroll
     for (int it = 0; it < 8; ++it) {
         const int group = w * 4 + (it >> 1), chunk = (it & 1) * 4 + (lane >> 3);
@@ -215,6 +318,14 @@ __device__ __forceinline__ void pp_store_tile(uint8_t *tile, const uint4 (&raw)[
         a.z = pg_e4m3x2_to_half2(r.y & 0xffffu), a.w = pg_e4m3x2_to_half2(r.y >> 16);
         b.x = pg_e4m3x2_to_half2(r.z & 0xffffu), b.y = pg_e4m3x2_to_half2(r.z >> 16);
         b.z = pg_e4m3x2_to_half2(r.w & 0xffffu), b.w = pg_e4m3x2_to_half2(r.w >> 16);
+        if constexpr (kScaled) {
+            const __half2 f = rel[it >> 2];
+            auto times = [&](uint32_t &x) {
+                const __half2 y = __hmul2(*reinterpret_cast<const __half2 *>(&x), f);
+                x = *reinterpret_cast<const uint32_t *>(&y);
+            };
+            times(a.x), times(a.y), times(a.z), times(a.w), times(b.x), times(b.y), times(b.z), times(b.w);
+        }
         *reinterpret_cast<uint4 *>(at) = a;
         *reinterpret_cast<uint4 *>(at + kPpSlice) = b;
     }
@@ -256,122 +367,143 @@ __device__ void pp_convert(const PaParams &p, PpShared &sm, int u0, int u1) {
         vref = fmaxf(fmaxf(sm.vmax[0], sm.vmax[1]), fmaxf(sm.vmax[2], sm.vmax[3]));
         if (!(vref > 0.0f)) vref = 1.0f;
         uint4 kr[8], vr[8];
-        auto load = [&](const void *codes, int i, uint4 (&r)[8]) {
-            const int key0 = s.span.step(s.off + i) * kPpKeys + w * 32 + (lane & 7);
+        // this thread's rows and columns in its two 16-position groups of tile i
+        long at[2];
+        int left[2];
+        auto place = [&](int i) {
+            const int j = s.span.step(s.off + i) * kPpKeys + w * 32;
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int page = __shfl_sync(0xffffffffu, pid, (i & 15) * 2 + half);
+            for (int g = 0; g < 2; ++g) {
+                const int page = __shfl_sync(0xffffffffu, pid, (i & 15) * 2 + g);
+                at[g] = (((long)page * p.c.kv_heads + s.h) * ps + ((j + 16 * g) & (ps - 1)) + (lane & 7)) * kPgDim +
+                        16 * (lane >> 3);
+                left[g] = page < 0 ? 0 : s.seq.len - (j + 16 * g + (lane & 7));  // > 8 u: row u of it is in the sequence
+            }
+        };
+        auto load = [&](const void *codes, uint4 (&r)[8]) {
+            const uint8_t *base = static_cast<const uint8_t *>(codes);
 #pragma unroll
-                for (int it = half * 4; it < half * 4 + 4; ++it) {
-                    const int key = key0 + (it >> 1) * 8, chunk = (it & 1) * 4 + (lane >> 3);
-                    r[it] = make_uint4(0u, 0u, 0u, 0u);
-                    // slots past the sequence's end may hold anything
-                    if (page >= 0 && key < s.seq.len)
-                        r[it] = __ldg(reinterpret_cast<const uint4 *>(
-                                          static_cast<const uint8_t *>(codes) +
-                                          (((long)page * p.c.kv_heads + s.h) * ps + (key & (ps - 1))) * kPgDim) +
-                                      chunk);
-                }
+            for (int it = 0; it < 8; ++it) {
+                const int g = it >> 2, u = (it >> 1) & 1;
+                r[it] = make_uint4(0u, 0u, 0u, 0u);  // slots past the sequence's end may hold anything
+                if (left[g] > 8 * u) r[it] = pp_ldg(base + at[g] + u * 8 * kPgDim + (it & 1) * 64);
             }
         };
         fetch(0);
-        load(p.c.k, 0, kr);
-        load(p.c.v, 0, vr);
+        place(0);
+        load(p.c.k, kr);
+        load(p.c.v, vr);
         for (int i = 0; ok && i < s.n; ++i, ++tile) {
             const int st = tile % kPpStages, use = tile / kPpStages;
             PpScale &sc = sm.sc[tile % kPpScales];
-            if ((lane >> 1) == (i & 15)) {
-                const int g = 2 * w + (lane & 1);
-                const float rel = fmaxf(log2f(vs / vref), kPpMinRel);
-                sc.k[g] = ks, sc.rel[g] = rel, sc.inv[g] = exp2f(-rel);
-            }
+            if ((lane >> 1) == (i & 15)) sc.k[2 * w + (lane & 1)] = ks;
+            const float ratio = vs / vref;
+            const __half2 rel[2] = {__float2half2_rn(__shfl_sync(0xffffffffu, ratio, (i & 15) * 2)),
+                                    __float2half2_rn(__shfl_sync(0xffffffffu, ratio, (i & 15) * 2 + 1))};
             if (w == 0 && lane == 0) sc.vref = vref;
             __syncwarp();
             if (lane == 0) mbar_arrive(&sm.sc_full[tile % kPpScales]);
             if (!(ok = pp_wait_warp(&sm.k_empty[st], (use & 1) ^ 1, sm, p))) break;
-            pp_store_tile(sm.k[st], kr, w, lane);
+            pp_store_tile<false>(sm.k[st], kr, w, lane, rel);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sm.k_full[st]);
             if (i + 1 < s.n) {
                 if (((i + 1) & 15) == 0) fetch(i + 1);
-                load(p.c.k, i + 1, kr);
+                place(i + 1);
+                load(p.c.k, kr);
             }
             if (!(ok = pp_wait_warp(&sm.v_empty[st], (use & 1) ^ 1, sm, p))) break;
-            pp_store_tile(sm.v[st], vr, w, lane);
+            pp_store_tile<true>(sm.v[st], vr, w, lane, rel);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sm.v_full[st]);
-            if (i + 1 < s.n) load(p.c.v, i + 1, vr);
+            if (i + 1 < s.n) load(p.c.v, vr);
         }
         u += s.n;
     }
 }
 
 // ---- warp 12: the products -----------------------------------------------------------------------
+// The whole warp walks the loops with values that the compiler can see to be uniform, and one
+// elected lane issues.  One warp issues for both row tiles, in turn: with a warp for each, the
+// products of the two interleave, both softmaxes get their scores at the same time, and then wait
+// for the products at the same time.
+__device__ __forceinline__ bool pp_elect() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e != 0;
+}
 __device__ void pp_products(const PaParams &p, PpShared &sm, int u0, int u1) {
     const int lane = threadIdx.x & 31;
-    const uint32_t tmem = sm.tmem;
-    int tile = 0, pieces[2] = {0, 0}, used[2] = {0, 0};  // tiles so far; pieces, tiles of each row tile
+    const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
     // K-major operands: 16-byte K slices kPpSlice apart, 8-row groups 128 apart; V (MN-major): 8-key
     // groups 128 apart, 8-column groups kPpSlice apart
-    auto scores = [&](int i, int st) {
-        const uint64_t a = umma_smem_desc(smem_u32(sm.q[i]), kPpSlice, 128);
-        const uint64_t b = umma_smem_desc(smem_u32(sm.k[st]), kPpSlice, 128);
+    const uint32_t q0 = pp_desc_lo(smem_u32(sm.q[0]), kPpSlice);
+    const uint32_t k0 = pp_desc_lo(smem_u32(sm.k[0]), kPpSlice), v0 = pp_desc_lo(smem_u32(sm.v[0]), 128);
+    auto scores = [&](int i, int st, bool last) {
+        const uint32_t a = q0 + i * (kPpTile >> 4), b = k0 + st * (kPpTile >> 4);
+        if (pp_elect()) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-            pp_mma_ss(tmem + kColS + 128 * i, a + (uint64_t)(k * 2 * kPpSlice >> 4), b + (uint64_t)(k * 2 * kPpSlice >> 4),
-                      kPpIdesc, k > 0);
-        tc_commit(&sm.s_full[i]);
+            for (int k = 0; k < 8; ++k)
+                pp_mma_ss(tmem + kColS + 128 * i, a + (k * 2 * kPpSlice >> 4), pp_desc_hi(128), b + (k * 2 * kPpSlice >> 4),
+                          pp_desc_hi(128), kPpIdesc, k > 0);
+            tc_commit(&sm.s_full[i]);
+            if (last) tc_commit(&sm.k_empty[st]);
+        }
+        __syncwarp();
     };
-    auto values = [&](int i, int st, bool first) {
-        const uint64_t b = umma_smem_desc(smem_u32(sm.v[st]), 128, kPpSlice);
+    auto values = [&](int i, int st, int half, bool first, bool last) {
+        const uint32_t b = v0 + st * (kPpTile >> 4) + half * (4 * 256 >> 4);
+        if (pp_elect()) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-            pp_mma_ts(tmem + kColO + 128 * i, tmem + kColS + 128 * i + 8 * k, b + (uint64_t)(k * 256 >> 4), kPpIdescV,
-                      !(first && k == 0));
-        tc_commit(&sm.o_done[i]);
+            for (int k = 0; k < 4; ++k)
+                pp_mma_ts(tmem + kColO + 128 * i, tmem + kColS + 128 * i + 32 * half + 8 * k, b + (k * 256 >> 4),
+                          pp_desc_hi(kPpSlice), kPpIdescV, !(first && k == 0 && half == 0));
+            if (half) tc_commit(&sm.o_done[i]);
+            if (half && last) tc_commit(&sm.v_empty[st]);
+        }
+        __syncwarp();
     };
     bool ok = true;
+    auto wait = [&](uint64_t *bar, int use) {
+        ok = ok && pp_wait_warp(bar, (uint32_t)use & 1, sm, p);
+        tc_fence_after();
+        return ok;
+    };
+    int tile = 0, pieces[2] = {0, 0}, used[2] = {0, 0};  // tiles so far; pieces, tiles of each row tile
     for (int u = u0; ok && u < u1;) {
         PpSeg s;
         pp_seek(p, sm, u, u1, lane, s);
-        const int tiles = s.rows > 128 ? 2 : 1;
-        if (lane == 0) {
-            auto wait = [&](uint64_t *bar, int use) {
-                ok = ok && pp_wait(bar, (uint32_t)use & 1, sm, p);
-                tc_fence_after();
-                return ok;
-            };
-            wait(&sm.k_full[tile % kPpStages], tile / kPpStages);
-            for (int i = 0; i < tiles; ++i)
-                if (wait(&sm.q_full[i], pieces[i])) scores(i, tile % kPpStages);
-            if (ok) tc_commit(&sm.k_empty[tile % kPpStages]);
-            for (int j = 0; ok && j < s.n; ++j) {
-                const int at = tile + j, st = at % kPpStages, next = (at + 1) % kPpStages;
-                wait(&sm.v_full[st], at / kPpStages);
-                for (int i = 0; i < tiles; ++i) {
-                    if (!wait(&sm.p_full[i], used[i] + j)) break;
-                    values(i, st, j == 0);
-                    if (i == tiles - 1) tc_commit(&sm.v_empty[st]);
-                    if (j + 1 == s.n) continue;
-                    // the products end in the order of their issue: P is read before S's next tile
-                    // overwrites it
-                    if (i == 0 && !wait(&sm.k_full[next], (at + 1) / kPpStages)) break;
-                    scores(i, next);
-                    if (i == tiles - 1) tc_commit(&sm.k_empty[next]);
-                }
+        const int n = __shfl_sync(0xffffffffu, s.n, 0);
+        const bool two = s.rows > 128;
+        wait(&sm.k_full[tile % kPpStages], tile / kPpStages);
+        if (wait(&sm.q_full[0], pieces[0])) scores(0, tile % kPpStages, !two);
+        if (two && wait(&sm.q_full[1], pieces[1])) scores(1, tile % kPpStages, true);
+        for (int j = 0; ok && j < n; ++j) {
+            const int at = tile + j, st = at % kPpStages, next = (at + 1) % kPpStages;
+            const bool more = j + 1 < n;
+            wait(&sm.v_full[st], at / kPpStages);
+            if (more) wait(&sm.k_full[next], (at + 1) / kPpStages);
+            for (int i = 0; ok && i < (two ? 2 : 1); ++i) {
+                const bool last = i == 1 || !two;
+                if (!wait(&sm.p_half[i], used[i] + j)) break;
+                values(i, st, 0, j == 0, last);
+                if (!wait(&sm.p_full[i], used[i] + j)) break;
+                values(i, st, 1, j == 0, last);
+                // the products end in the order of their issue: P is read before S's next tile
+                // overwrites it
+                if (more) scores(i, next, last);
             }
         }
-        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-        tile += s.n;
-        for (int i = 0; i < tiles; ++i) ++pieces[i], used[i] += s.n;
-        u += s.n;
+        tile += n;
+        ++pieces[0], used[0] += n;
+        if (two) ++pieces[1], used[1] += n;
+        u += n;
     }
-    if (lane == 0) {  // every product has ended before the tensor memory goes
-        tc_commit(&sm.mdone);
-        mbar_wait_bounded(&sm.mdone, 0, globaltimer_ns() + kPaTimeoutNs);
-    }
+    if (pp_elect()) tc_commit(&sm.mdone);  // every product has ended before the tensor memory goes
+    __syncwarp();
+    mbar_wait_bounded(&sm.mdone, 0, globaltimer_ns() + kPaTimeoutNs);
     __syncwarp();
 }
 
@@ -424,14 +556,18 @@ __device__ void pp_softmax(const PaParams &p, PpShared &sm, int u0, int u1, int 
     const int row = (warp & 3) * 32 + lane;  // row of the tile, and lane of the tensor memory
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = sm.tmem + lanes + kColS + 128 * i, to = sm.tmem + lanes + kColO + 128 * i;
-    int tile = 0, used = 0;
+    // The two row tiles take turns at the exponentials: left alone, both softmaxes share the units, end
+    // together and then wait together for the products.  Tile 0's k-th turn follows tile 1's k-1st,
+    // tile 1's k-th follows tile 0's.
+    int tile = 0, used = 0, turns = 0;
     bool ok = true;  // after a failed wait only the barriers among these warps go on
     for (int u = u0; u < u1;) {
         PpSeg s;
         pp_seek(p, sm, u, u1, lane, s);
         const int end = u - s.off + s.nb, c0 = (u - s.off) / share, c1 = (end - 1) / share;
         float *slot = p.partials + ((size_t)blockIdx.x * 2 + ((int)blockIdx.x == c0 ? 1 : 0)) * kPpSlotFloats;
-        if (ok && (i == 0 || s.rows > 128)) {
+        const bool two = s.rows > 128;
+        if (ok && (i == 0 || two)) {
             const int r = i * 128 + row;  // of the item
             const bool live = r < s.rows, warp_live = i * 128 + (warp & 3) * 32 < s.rows;
             const int pos = live ? s.seq.pos0 + (s.row0 + r) / p.group : -1;
@@ -443,43 +579,48 @@ __device__ void pp_softmax(const PaParams &p, PpShared &sm, int u0, int u1, int 
             if (lane == 0) mbar_arrive(&sm.q_full[i]);
             for (int j = 0; j < s.n; ++j) {
                 const int at = tile + j;
-                ok = pp_wait_warp(&sm.s_full[i], (uint32_t)(used + j) & 1, sm, p) &&
-                     pp_wait_warp(&sm.sc_full[at % kPpScales], (uint32_t)(at / kPpScales) & 1, sm, p);
+                const PpScale &sc = sm.sc[at % kPpScales];
+                ok = pp_wait_warp(&sm.sc_full[at % kPpScales], (uint32_t)(at / kPpScales) & 1, sm, p);
+                const int key0 = s.span.step(s.off + j) * kPpKeys;
+                bool whole = key0 + kPpKeys - 1 <= pos &&
+                             (p.window <= 0 || pos - key0 < p.window || key0 + kPpKeys <= p.sinks);
+                // the tile's scales into registers while the scores are under way (a read of shared memory
+                // in the loops below waits behind the products' operands)
+                float col[8], least = INFINITY;
+#pragma unroll
+                for (int g = 0; g < 8; g += 4)
+                    *reinterpret_cast<float4 *>(col + g) = *reinterpret_cast<const float4 *>(sc.k + g);
+                vref = sc.vref;
+#pragma unroll
+                for (int g = 0; g < 8; ++g) {
+                    least = fminf(least, col[g]);
+                    // a column's factor: never 0, so that a masked score's -infinity stays one
+                    col[g] = fmaxf(col[g] * factor, 1e-35f);
+                }
+                whole = whole & !(least < 0.0f);
+                whole = __all_sync(0xffffffffu, whole);
+                ok = ok && pp_wait_warp(&sm.s_full[i], (uint32_t)(used + j) & 1, sm, p);
                 if (!ok) break;
                 tc_fence_after();
                 if (warp_live) {
-                    const PpScale &sc = sm.sc[at % kPpScales];
-                    const int key0 = s.span.step(s.off + j) * kPpKeys;
-                    vref = sc.vref;
-                    bool whole = key0 + kPpKeys - 1 <= pos &&
-                                 (p.window <= 0 || pos - key0 < p.window || key0 + kPpKeys <= p.sinks);
-                    float col[8];
-#pragma unroll
-                    for (int g = 0; g < 8; ++g) {
-                        whole = whole && !(sc.k[g] < 0.0f);
-                        col[g] = sc.k[g] * factor;
-                    }
-                    whole = __all_sync(0xffffffffu, whole);
-                    auto sees = [&](int g, int x) {
-                        return !(sc.k[g] < 0.0f) && pa_sees(key0 + g * 16 + x, pos, p.window, p.sinks);
-                    };
+                    if (!whole) pp_mask(ts, pos - key0, p.window, p.sinks - key0, sc.k);
+                    // S is read twice, 32 columns at a time and one read ahead, so that a row needs 64
+                    // registers for it and nothing is spilled (128 columns at once were: the spills'
+                    // reloads missed an L1 that the codes stream through)
+                    float v[2][32];
                     float top = -INFINITY;
+                    pp_ld32(ts, v[0]);
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        float v[32];
-                        pp_ld32(ts + 32 * c, v);
-                        pp_wait_ld(v);
+                        float(&x)[32] = v[c & 1];
+                        pp_wait_ld(x);
+                        pp_ld32(ts + 32 * ((c + 1) & 3), v[(c + 1) & 1]);
 #pragma unroll
                         for (int g = 0; g < 2; ++g) {
-                            float mx = -INFINITY;
-                            if (whole) {
+                            float mx = x[16 * g];
 #pragma unroll
-                                for (int x = 0; x < 16; ++x) mx = fmaxf(mx, v[16 * g + x]);
-                            } else {
-#pragma unroll
-                                for (int x = 0; x < 16; ++x) mx = sees(2 * c + g, x) ? fmaxf(mx, v[16 * g + x]) : mx;
-                            }
-                            if (mx != -INFINITY) top = fmaxf(top, mx * col[2 * c + g]);
+                            for (int y = 1; y < 16; ++y) mx = fmaxf(mx, x[16 * g + y]);
+                            top = fmaxf(top, mx * col[2 * c + g]);
                         }
                     }
                     const bool grows = top > m + kPpLazy || (m == -INFINITY && top != -INFINITY);
@@ -491,59 +632,70 @@ __device__ void pp_softmax(const PaParams &p, PpShared &sm, int u0, int u1, int 
                         l *= f;
                         if (!(ok = pp_wait_warp(&sm.o_done[i], (uint32_t)(used + j - 1) & 1, sm, p))) break;
                         tc_fence_after();
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            float v[32];
-                            pp_ld32(to + 32 * c, v);
-                            pp_wait_ld(v);
-                            uint32_t w[2][16];
-#pragma unroll
-                            for (int x = 0; x < 32; ++x) w[x >> 4][x & 15] = __float_as_uint(v[x] * f);
-                            pp_st16(to + 32 * c, w[0]);
-                            pp_st16(to + 32 * c + 16, w[1]);
-                        }
-                        pp_wait_st();
+                        pp_scale_o(to, f);
                     }
                     const float base = m == -INFINITY ? 0.0f : m;
+                    const uint64_t less = pp_pair(-base, -base);
+                    uint64_t sum = 0;
+                    if (two && !(ok = pp_wait_warp(&sm.turn[i], (uint32_t)(turns + j + 1 - i) & 1, sm, p))) break;
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        float v[32];
-                        pp_ld32(ts + 32 * c, v);
-                        pp_wait_ld(v);
+                        float(&x)[32] = v[c & 1];
+                        pp_wait_ld(x);
+                        if (c < 3) pp_ld32(ts + 32 * (c + 1), v[(c + 1) & 1]);
                         uint32_t w[16];
 #pragma unroll
                         for (int g = 0; g < 2; ++g) {
-                            const float add = sc.rel[2 * c + g] - base;
-                            float sum = 0.0f;
+                            const uint64_t col2 = pp_pair(col[2 * c + g], col[2 * c + g]);
 #pragma unroll
-                            for (int x = 0; x < 16; x += 2) {
-                                float e0 = pa_exp2(fmaf(v[16 * g + x], col[2 * c + g], add));
-                                float e1 = pa_exp2(fmaf(v[16 * g + x + 1], col[2 * c + g], add));
-                                if (!whole) {
-                                    e0 = sees(2 * c + g, x) ? e0 : 0.0f;
-                                    e1 = sees(2 * c + g, x + 1) ? e1 : 0.0f;
+                            for (int y = 16 * g; y < 16 * g + 16; y += 2) {
+                                float e0, e1;
+                                uint64_t e = pp_fma2(pp_pair(x[y], x[y + 1]), col2, less);
+                                if (y % 8 == 6) {
+                                    e = pp_exp2_fma(e);
+                                    pp_split(e, e0, e1);
+                                } else {
+                                    pp_split(e, e0, e1);
+                                    e0 = pa_exp2(e0), e1 = pa_exp2(e1);
+                                    e = pp_pair(e0, e1);
                                 }
-                                sum += e0 + e1;
-                                w[8 * g + x / 2] = pg_pack2(e0, e1, (const __half *)nullptr);
+                                sum = pp_add2(sum, e);
+                                w[y / 2] = pg_pack2(e0, e1, (const __half *)nullptr);
                             }
-                            l += sum * sc.inv[2 * c + g];
                         }
                         pp_st16(ts + 16 * c, w);  // these columns of S have been read
+                        if (c == 1) {  // P's first half: its product can begin
+                            pp_wait_st();
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(&sm.p_half[i]);
+                        }
                     }
+                    float s0, s1;
+                    pp_split(sum, s0, s1);
+                    l += s0 + s1;
+                    __syncwarp();
+                    if (two && lane == 0) mbar_arrive(&sm.turn[1 - i]);
                     pp_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sm.p_full[i]);
+                } else if (lane == 0) {
+                    mbar_arrive(&sm.p_half[i]);
+                    if (two) mbar_arrive(&sm.turn[1 - i]);
+                    mbar_arrive(&sm.p_full[i]);
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sm.p_full[i]);
             }
             ok = ok && pp_wait_warp(&sm.o_done[i], (uint32_t)(used + s.n - 1) & 1, sm, p);
             tc_fence_after();
             used += s.n;
+            if (two) turns += s.n;
             if (ok && warp_live) {
                 const long dst = (long)(s.seq.row0 + (s.row0 + r) / p.group) * p.query_heads + s.h * p.group +
                                  (s.row0 + r) % p.group;
-                const float f = c0 != c1 ? vref : l == 0.0f ? 0.0f : vref / l;
-#pragma unroll
+                const bool none = m == -INFINITY && l == l;  // the row saw nothing (a NaN score leaves l NaN)
+                const float f = c0 != c1 ? vref : none ? 0.0f : vref / l;
+#pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
                     float v[32];
                     pp_ld32(to + 32 * c, v);
@@ -560,7 +712,7 @@ __device__ void pp_softmax(const PaParams &p, PpShared &sm, int u0, int u1, int 
                     }
                 }
                 if (live && c0 == c1) {
-                    if (p.lse) p.lse[dst] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kPaLn2;
+                    if (p.lse) p.lse[dst] = none ? -INFINITY : (m + log2f(l)) * kPaLn2;
                 } else if (live) {
                     slot[(size_t)kPpRows * kPgDim + r] = m;
                     slot[(size_t)kPpRows * (kPgDim + 1) + r] = l;
@@ -593,11 +745,12 @@ __device__ void pp_softmax(const PaParams &p, PpShared &sm, int u0, int u1, int 
                     }
                     const long dst = (long)(s.seq.row0 + (s.row0 + r) / p.group) * p.query_heads + s.h * p.group +
                                      (s.row0 + r) % p.group;
-                    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                    const bool none = top == -INFINITY && l == l;
+                    const float inv = none ? 0.0f : 1.0f / l;
                     T *out = static_cast<T *>(p.out) + dst * kPgDim;
                     reinterpret_cast<uint2 *>(out)[lane] =
                         make_uint2(pg_pack2(acc.x * inv, acc.y * inv, out), pg_pack2(acc.z * inv, acc.w * inv, out));
-                    if (p.lse && lane == 0) p.lse[dst] = l == 0.0f ? -INFINITY : (top + log2f(l)) * kPaLn2;
+                    if (p.lse && lane == 0) p.lse[dst] = none ? -INFINITY : (top + log2f(l)) * kPaLn2;
                 }
                 if (threadIdx.x == 0) p.counters[c0] = 0u;
             }
@@ -614,7 +767,8 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_attend_prompt_kernel(cons
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&sm.q_full[i], 4), mbar_init(&sm.p_full[i], 4);
+            mbar_init(&sm.q_full[i], 4), mbar_init(&sm.turn[i], 4);
+            mbar_init(&sm.p_half[i], 4), mbar_init(&sm.p_full[i], 4);
             mbar_init(&sm.s_full[i], 1), mbar_init(&sm.o_done[i], 1);
         }
         for (int i = 0; i < kPpStages; ++i) {
@@ -657,9 +811,17 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_attend_prompt_kernel(cons
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp < kPpConvWarp0) pp_softmax<T>(p, sm, u0, u1, share);
-    else if (warp < kPpMmaWarp) pp_convert(p, sm, u0, u1);
-    else pp_products(p, sm, u0, u1);
+    // launched with 128 registers a thread: 256 x 160 + 128 x 112 + 128 x 80 = 512 x 128
+    if (warp < kPpConvWarp0) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
+        pp_softmax<T>(p, sm, u0, u1, share);
+    } else if (warp < kPpMmaWarp) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 112;");
+        pp_convert(p, sm, u0, u1);
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        if (warp == kPpMmaWarp) pp_products(p, sm, u0, u1);
+    }
     tc_fence_before();
     __syncthreads();
     if (warp == kPpMmaWarp) {
