@@ -51,7 +51,7 @@ struct PpShared {
     PpScale sc[kPpScales];
     float vmax[4];
     int prefix[kPaMaxSeqs + 1];
-    uint64_t q_full[2], s_full[2], p_half[2], p_full[2], o_done[2], turn[2];
+    uint64_t q_full[2], s_full[2][2], p_full[2][2], o_done[2][2];  // [row tile][half]
     uint64_t k_full[kPpStages], k_empty[kPpStages], v_full[kPpStages], v_empty[kPpStages], sc_full[kPpScales];
     uint64_t mdone;
     uint32_t tmem;
@@ -61,7 +61,8 @@ constexpr size_t kPpSmem = sizeof(PpShared) + 128;
 static_assert(kPpSmem <= 227 * 1024, "shared memory");
 
 constexpr uint32_t kPpIdesc = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);  // f16 x f16 -> f32, 128 x 128
-constexpr uint32_t kPpIdescV = kPpIdesc | (1u << 16);                                 // B read MN-major
+constexpr uint32_t kPpIdescV = kPpIdesc | (1u << 16);  // B read MN-major
+constexpr uint32_t kPpIdescS = (1u << 4) | ((64u >> 3) << 17) | ((128u >> 4) << 24);  // 128 x 64
 constexpr uint32_t kColS = 0, kColO = 256;
 
 // Descriptors as their 32-bit halves (umma_smem_desc): only the low one moves with the address.
@@ -167,7 +168,7 @@ __device__ __forceinline__ void pp_wait_st() { asm volatile("tcgen05.wait::st.sy
 __device__ __forceinline__ void pp_mask(uint32_t ts, int at, int window, int first, const float *ks) {
     const int gone = window > 0 ? at - window : -1, seen = window > 0 ? first : 0;
 #pragma unroll 1
-    for (int c = 0; c < 4; ++c) {
+    for (int c = 0; c < 2; ++c) {
         float v[32];
         pp_ld32(ts + 32 * c, v);
         const bool none0 = ks[2 * c] < 0.0f, none1 = ks[2 * c + 1] < 0.0f;
@@ -201,29 +202,25 @@ __device__ __forceinline__ void pp_scale_o(uint32_t to, float f) {
     pp_wait_st();
 }
 
-// Bounded wait of one role: false when two seconds have passed or another role has given up.
+// Bounded wait of one role: false when about two seconds have passed (2^20 sleeps of at most 2 us) or
+// another role has given up.  The warp sleeps in hardware until the phase ends: a spinning one takes
+// the path that the exponentials and shared memory need.
 __device__ __forceinline__ bool pp_wait(uint64_t *bar, uint32_t parity, PpShared &sm, const PaParams &p) {
     if (mbar_test_wait(bar, parity)) return true;
-    // the warp sleeps in hardware until the phase ends: a spinning one takes the path that the
-    // exponentials and shared memory need
-    uint64_t start = 0;
-    for (;;) {
+#pragma unroll 1
+    for (int n = 0; n < (1 << 20); ++n) {
         uint32_t ok;
         asm volatile(
             "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
             : "=r"(ok)
-            : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)
+            : "r"(smem_u32(bar)), "r"(parity), "r"(2000u)
             : "memory");
         if (ok) return true;
         if (*reinterpret_cast<volatile int *>(&sm.abort)) return false;
-        const uint64_t now = globaltimer_ns();
-        if (start == 0) start = now;
-        if (now - start > kPaTimeoutNs) {
-            *reinterpret_cast<volatile int *>(&sm.abort) = 1;
-            atomicExch(p.status, (uint32_t)MMRS_ERR_TIMEOUT);
-            return false;
-        }
     }
+    *reinterpret_cast<volatile int *>(&sm.abort) = 1;
+    atomicExch(p.status, (uint32_t)MMRS_ERR_TIMEOUT);
+    return false;
 }
 
 // The same for a whole warp, with one answer.
@@ -250,6 +247,7 @@ __device__ int pp_seq_units(const PaParams &p, const PgSeq &seq, int lane) {
     const int tiles = (seq.count * p.group + kPpRows - 1) / kPpRows;
     int sum = 0;
     PaSpan<kPpKeys> span;
+#pragma unroll 1
     for (int rt = lane; rt < tiles; rt += 32) sum += pp_tiles(p, seq, rt, span);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -271,6 +269,7 @@ __device__ void pp_seek(const PaParams &p, const PpShared &sm, int u, int end, i
     at -= s.h * per_head;
     const int tiles = (s.seq.count * p.group + kPpRows - 1) / kPpRows;
     int rt = 0, before = 0;
+#pragma unroll 1
     for (int r0 = 0; r0 < tiles; r0 += 32) {
         PaSpan<kPpKeys> span;
         const int n = r0 + lane < tiles ? pp_tiles(p, s.seq, r0 + lane, span) : 0;
@@ -335,6 +334,7 @@ __device__ void pp_convert(const PaParams &p, PpShared &sm, int u0, int u1) {
     const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) - kPpConvWarp0;
     int tile = 0;
     bool ok = true;  // after a failed wait only the barriers among these warps go on
+#pragma unroll 1
     for (int u = u0; u < u1;) {
         PpSeg s;
         pp_seek(p, sm, u, u1, lane, s);
@@ -356,6 +356,7 @@ __device__ void pp_convert(const PaParams &p, PpShared &sm, int u0, int u1) {
             }
         };
         float vref = 0.0f;
+#pragma unroll 1
         for (int base = 0; base < s.n; base += 16) {
             fetch(base);
             vref = fmaxf(vref, vs);
@@ -393,6 +394,7 @@ __device__ void pp_convert(const PaParams &p, PpShared &sm, int u0, int u1) {
         place(0);
         load(p.c.k, kr);
         load(p.c.v, vr);
+#pragma unroll 1
         for (int i = 0; ok && i < s.n; ++i, ++tile) {
             const int st = tile % kPpStages, use = tile / kPpStages;
             PpScale &sc = sm.sc[tile % kPpScales];
@@ -441,27 +443,28 @@ __device__ void pp_products(const PaParams &p, PpShared &sm, int u0, int u1) {
     // groups 128 apart, 8-column groups kPpSlice apart
     const uint32_t q0 = pp_desc_lo(smem_u32(sm.q[0]), kPpSlice);
     const uint32_t k0 = pp_desc_lo(smem_u32(sm.k[0]), kPpSlice), v0 = pp_desc_lo(smem_u32(sm.v[0]), 128);
-    auto scores = [&](int i, int st, bool last) {
-        const uint32_t a = q0 + i * (kPpTile >> 4), b = k0 + st * (kPpTile >> 4);
+    // half h of a tile: its 64 keys' scores, columns [64 h, 64 h + 64) of the row tile's S
+    auto scores = [&](int i, int st, int h, bool last) {
+        const uint32_t a = q0 + i * (kPpTile >> 4), b = k0 + st * (kPpTile >> 4) + h * (8 * 128 >> 4);
         if (pp_elect()) {
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-                pp_mma_ss(tmem + kColS + 128 * i, a + (k * 2 * kPpSlice >> 4), pp_desc_hi(128), b + (k * 2 * kPpSlice >> 4),
-                          pp_desc_hi(128), kPpIdesc, k > 0);
-            tc_commit(&sm.s_full[i]);
-            if (last) tc_commit(&sm.k_empty[st]);
+                pp_mma_ss(tmem + kColS + 128 * i + 64 * h, a + (k * 2 * kPpSlice >> 4), pp_desc_hi(128),
+                          b + (k * 2 * kPpSlice >> 4), pp_desc_hi(128), kPpIdescS, k > 0);
+            tc_commit(&sm.s_full[i][h]);
+            if (h && last) tc_commit(&sm.k_empty[st]);
         }
         __syncwarp();
     };
-    auto values = [&](int i, int st, int half, bool first, bool last) {
-        const uint32_t b = v0 + st * (kPpTile >> 4) + half * (4 * 256 >> 4);
+    auto values = [&](int i, int st, int h, bool first, bool last) {
+        const uint32_t b = v0 + st * (kPpTile >> 4) + h * (4 * 256 >> 4);
         if (pp_elect()) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                pp_mma_ts(tmem + kColO + 128 * i, tmem + kColS + 128 * i + 32 * half + 8 * k, b + (k * 256 >> 4),
-                          pp_desc_hi(kPpSlice), kPpIdescV, !(first && k == 0 && half == 0));
-            if (half) tc_commit(&sm.o_done[i]);
-            if (half && last) tc_commit(&sm.v_empty[st]);
+                pp_mma_ts(tmem + kColO + 128 * i, tmem + kColS + 128 * i + 64 * h + 8 * k, b + (k * 256 >> 4),
+                          pp_desc_hi(kPpSlice), kPpIdescV, !(first && k == 0));
+            tc_commit(&sm.o_done[i][h]);
+            if (h && last) tc_commit(&sm.v_empty[st]);
         }
         __syncwarp();
     };
@@ -472,29 +475,47 @@ __device__ void pp_products(const PaParams &p, PpShared &sm, int u0, int u1) {
         return ok;
     };
     int tile = 0, pieces[2] = {0, 0}, used[2] = {0, 0};  // tiles so far; pieces, tiles of each row tile
+#pragma unroll 1
     for (int u = u0; ok && u < u1;) {
         PpSeg s;
         pp_seek(p, sm, u, u1, lane, s);
         const int n = __shfl_sync(0xffffffffu, s.n, 0);
         const bool two = s.rows > 128;
         wait(&sm.k_full[tile % kPpStages], tile / kPpStages);
-        if (wait(&sm.q_full[0], pieces[0])) scores(0, tile % kPpStages, !two);
-        if (two && wait(&sm.q_full[1], pieces[1])) scores(1, tile % kPpStages, true);
-        for (int j = 0; ok && j < n; ++j) {
-            const int at = tile + j, st = at % kPpStages, next = (at + 1) % kPpStages;
+#pragma unroll 1
+        for (int x = 0; x < 4; ++x) {  // both halves of the first tile
+            const int i = x & 1, h = x >> 1;
+            if (i == 1 && !two) continue;
+            if (wait(&sm.q_full[i], pieces[i])) scores(i, tile % kPpStages, h, i == 1 || !two);
+        }
+        // A test of a barrier comes back late (it queues behind the softmaxes' exponentials), so each is
+        // asked ahead of its use and only a phase found open is waited for.
+        auto test = [&](uint64_t *bar, int use) { return mbar_test_wait(bar, (uint32_t)use & 1); };
+        bool p0 = false;
+#pragma unroll 1
+        for (int y = 0; ok && y < 2 * n; ++y) {
+            const int j = y >> 1, h = y & 1, at = tile + j, st = at % kPpStages, next = (at + 1) % kPpStages;
             const bool more = j + 1 < n;
-            wait(&sm.v_full[st], at / kPpStages);
-            if (more) wait(&sm.k_full[next], (at + 1) / kPpStages);
-            for (int i = 0; ok && i < (two ? 2 : 1); ++i) {
-                const bool last = i == 1 || !two;
-                if (!wait(&sm.p_half[i], used[i] + j)) break;
-                values(i, st, 0, j == 0, last);
-                if (!wait(&sm.p_full[i], used[i] + j)) break;
-                values(i, st, 1, j == 0, last);
-                // the products end in the order of their issue: P is read before S's next tile
-                // overwrites it
-                if (more) scores(i, next, last);
+            const bool v_in = test(&sm.v_full[st], at / kPpStages);
+            const bool k_in = !more || test(&sm.k_full[next], (at + 1) / kPpStages);
+            if (!p0) p0 = test(&sm.p_full[0][h], used[0] + j);
+            bool p1 = two && test(&sm.p_full[1][h], used[1] + j);
+            if (!__all_sync(0xffffffffu, v_in && k_in && p0)) {
+                wait(&sm.v_full[st], at / kPpStages);
+                if (more) wait(&sm.k_full[next], (at + 1) / kPpStages);
+                if (!wait(&sm.p_full[0][h], used[0] + j)) break;
             }
+            tc_fence_after();
+            values(0, st, h, y == 0, !two);
+            // the products end in the order of their issue: P is read before the scores of the next tile's
+            // half overwrite it
+            if (more) scores(0, next, h, !two);
+            p0 = y + 1 < 2 * n && test(&sm.p_full[0][h ^ 1], used[0] + ((y + 1) >> 1));
+            if (!two) continue;
+            if (!__all_sync(0xffffffffu, p1) && !wait(&sm.p_full[1][h], used[1] + j)) break;
+            tc_fence_after();
+            values(1, st, h, y == 0, true);
+            if (more) scores(1, next, h, true);
         }
         tile += n;
         ++pieces[0], used[0] += n;
@@ -556,11 +577,9 @@ __device__ void pp_softmax(const PaParams &p, PpShared &sm, int u0, int u1, int 
     const int row = (warp & 3) * 32 + lane;  // row of the tile, and lane of the tensor memory
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = sm.tmem + lanes + kColS + 128 * i, to = sm.tmem + lanes + kColO + 128 * i;
-    // The two row tiles take turns at the exponentials: left alone, both softmaxes share the units, end
-    // together and then wait together for the products.  Tile 0's k-th turn follows tile 1's k-1st,
-    // tile 1's k-th follows tile 0's.
-    int tile = 0, used = 0, turns = 0;
+    int tile = 0, used = 0;
     bool ok = true;  // after a failed wait only the barriers among these warps go on
+#pragma unroll 1
     for (int u = u0; u < u1;) {
         PpSeg s;
         pp_seek(p, sm, u, u1, lane, s);
@@ -577,81 +596,75 @@ __device__ void pp_softmax(const PaParams &p, PpShared &sm, int u0, int u1, int 
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sm.q_full[i]);
-            for (int j = 0; j < s.n; ++j) {
-                const int at = tile + j;
+#pragma unroll 1
+            for (int y = 0; y < 2 * s.n; ++y) {
+                const int j = y >> 1, h = y & 1, at = tile + j;
                 const PpScale &sc = sm.sc[at % kPpScales];
-                ok = pp_wait_warp(&sm.sc_full[at % kPpScales], (uint32_t)(at / kPpScales) & 1, sm, p);
-                const int key0 = s.span.step(s.off + j) * kPpKeys;
-                bool whole = key0 + kPpKeys - 1 <= pos &&
-                             (p.window <= 0 || pos - key0 < p.window || key0 + kPpKeys <= p.sinks);
-                // the tile's scales into registers while the scores are under way (a read of shared memory
-                // in the loops below waits behind the products' operands)
-                float col[8], least = INFINITY;
-#pragma unroll
-                for (int g = 0; g < 8; g += 4)
-                    *reinterpret_cast<float4 *>(col + g) = *reinterpret_cast<const float4 *>(sc.k + g);
-                vref = sc.vref;
-#pragma unroll
-                for (int g = 0; g < 8; ++g) {
-                    least = fminf(least, col[g]);
-                    // a column's factor: never 0, so that a masked score's -infinity stays one
-                    col[g] = fmaxf(col[g] * factor, 1e-35f);
-                }
-                whole = whole & !(least < 0.0f);
-                whole = __all_sync(0xffffffffu, whole);
-                ok = ok && pp_wait_warp(&sm.s_full[i], (uint32_t)(used + j) & 1, sm, p);
+                const uint32_t tsh = ts + 64 * h;
+                // the scales were written before the products of this tile were issued: both tests in one go
+                uint64_t *sc_bar = &sm.sc_full[at % kPpScales];
+                const bool there = mbar_test_wait(sc_bar, (uint32_t)(at / kPpScales) & 1);
+                ok = pp_wait_warp(&sm.s_full[i][h], (uint32_t)(used + j) & 1, sm, p);
+                if (!__all_sync(0xffffffffu, there)) ok = ok && pp_wait_warp(sc_bar, (uint32_t)(at / kPpScales) & 1, sm, p);
                 if (!ok) break;
                 tc_fence_after();
                 if (warp_live) {
-                    if (!whole) pp_mask(ts, pos - key0, p.window, p.sinks - key0, sc.k);
-                    // S is read twice, 32 columns at a time and one read ahead, so that a row needs 64
-                    // registers for it and nothing is spilled (128 columns at once were: the spills'
-                    // reloads missed an L1 that the codes stream through)
                     float v[2][32];
+                    pp_ld32(tsh, v[0]);
+                    pp_ld32(tsh + 32, v[1]);
+                    float4 ks = *reinterpret_cast<const float4 *>(sc.k + 4 * h);
+                    vref = sc.vref;
+                    const int key0 = s.span.step(s.off + j) * kPpKeys + 64 * h;
+                    const bool whole = key0 + 63 <= pos &&
+                                       (p.window <= 0 || pos - key0 < p.window || key0 + 64 <= p.sinks) &
+                                           !(fminf(fminf(ks.x, ks.y), fminf(ks.z, ks.w)) < 0.0f);
+                    pp_wait_ld(v[0]);
+                    pp_hold32(v[1]);
+                    if (!__all_sync(0xffffffffu, whole)) {
+                        pp_mask(tsh, pos - key0, p.window, p.sinks - key0, sc.k + 4 * h);
+                        pp_ld32(tsh, v[0]);
+                        pp_ld32(tsh + 32, v[1]);
+                        pp_wait_ld(v[0]);
+                        pp_hold32(v[1]);
+                    }
+                    // a column's factor: never 0, so that a masked score's -infinity stays one
+                    const float col[4] = {fmaxf(ks.x * factor, 1e-35f), fmaxf(ks.y * factor, 1e-35f),
+                                          fmaxf(ks.z * factor, 1e-35f), fmaxf(ks.w * factor, 1e-35f)};
                     float top = -INFINITY;
-                    pp_ld32(ts, v[0]);
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        float(&x)[32] = v[c & 1];
-                        pp_wait_ld(x);
-                        pp_ld32(ts + 32 * ((c + 1) & 3), v[(c + 1) & 1]);
+                    for (int g = 0; g < 4; ++g) {
+                        const float *x = &v[g >> 1][16 * (g & 1)];
+                        float mx = x[0], my = x[8];
 #pragma unroll
-                        for (int g = 0; g < 2; ++g) {
-                            float mx = x[16 * g];
-#pragma unroll
-                            for (int y = 1; y < 16; ++y) mx = fmaxf(mx, x[16 * g + y]);
-                            top = fmaxf(top, mx * col[2 * c + g]);
-                        }
+                        for (int c = 1; c < 8; ++c) mx = fmaxf(mx, x[c]), my = fmaxf(my, x[8 + c]);
+                        top = fmaxf(top, fmaxf(mx, my) * col[g]);
                     }
                     const bool grows = top > m + kPpLazy || (m == -INFINITY && top != -INFINITY);
-                    if (j == 0) {
+                    if (y == 0) {
                         m = top;
                     } else if (__any_sync(0xffffffffu, grows)) {
                         const float now = fmaxf(m, top), f = now == -INFINITY ? 1.0f : pa_exp2(m - now);
                         m = now;
                         l *= f;
-                        if (!(ok = pp_wait_warp(&sm.o_done[i], (uint32_t)(used + j - 1) & 1, sm, p))) break;
+                        if (!(ok = pp_wait_warp(&sm.o_done[i][h ^ 1], (uint32_t)(used + ((y - 1) >> 1)) & 1, sm, p))) break;
                         tc_fence_after();
                         pp_scale_o(to, f);
                     }
                     const float base = m == -INFINITY ? 0.0f : m;
                     const uint64_t less = pp_pair(-base, -base);
                     uint64_t sum = 0;
-                    if (two && !(ok = pp_wait_warp(&sm.turn[i], (uint32_t)(turns + j + 1 - i) & 1, sm, p))) break;
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        float(&x)[32] = v[c & 1];
-                        pp_wait_ld(x);
-                        if (c < 3) pp_ld32(ts + 32 * (c + 1), v[(c + 1) & 1]);
+                    for (int c = 0; c < 2; ++c) {
+                        const float(&x)[32] = v[c];
                         uint32_t w[16];
 #pragma unroll
                         for (int g = 0; g < 2; ++g) {
                             const uint64_t col2 = pp_pair(col[2 * c + g], col[2 * c + g]);
 #pragma unroll
-                            for (int y = 16 * g; y < 16 * g + 16; y += 2) {
+                            for (int z = 16 * g; z < 16 * g + 16; z += 2) {
                                 float e0, e1;
-                                uint64_t e = pp_fma2(pp_pair(x[y], x[y + 1]), col2, less);
-                                if (y % 8 == 6) {
+                                uint64_t e = pp_fma2(pp_pair(x[z], x[z + 1]), col2, less);
+                                if (z % 8 == 6) {
                                     e = pp_exp2_fma(e);
                                     pp_split(e, e0, e1);
                                 } else {
@@ -660,36 +673,23 @@ __device__ void pp_softmax(const PaParams &p, PpShared &sm, int u0, int u1, int 
                                     e = pp_pair(e0, e1);
                                 }
                                 sum = pp_add2(sum, e);
-                                w[y / 2] = pg_pack2(e0, e1, (const __half *)nullptr);
+                                w[z / 2] = pg_pack2(e0, e1, (const __half *)nullptr);
                             }
                         }
-                        pp_st16(ts + 16 * c, w);  // these columns of S have been read
-                        if (c == 1) {  // P's first half: its product can begin
-                            pp_wait_st();
-                            tc_fence_before();
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive(&sm.p_half[i]);
-                        }
+                        pp_st16(tsh + 16 * c, w);  // this half of S has been read
                     }
                     float s0, s1;
                     pp_split(sum, s0, s1);
                     l += s0 + s1;
-                    __syncwarp();
-                    if (two && lane == 0) mbar_arrive(&sm.turn[1 - i]);
                     pp_wait_st();
                     tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sm.p_full[i]);
-                } else if (lane == 0) {
-                    mbar_arrive(&sm.p_half[i]);
-                    if (two) mbar_arrive(&sm.turn[1 - i]);
-                    mbar_arrive(&sm.p_full[i]);
                 }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.p_full[i][h]);
             }
-            ok = ok && pp_wait_warp(&sm.o_done[i], (uint32_t)(used + s.n - 1) & 1, sm, p);
+            ok = ok && pp_wait_warp(&sm.o_done[i][1], (uint32_t)(used + s.n - 1) & 1, sm, p);
             tc_fence_after();
             used += s.n;
-            if (two) turns += s.n;
             if (ok && warp_live) {
                 const long dst = (long)(s.seq.row0 + (s.row0 + r) / p.group) * p.query_heads + s.h * p.group +
                                  (s.row0 + r) % p.group;
@@ -729,6 +729,7 @@ __device__ void pp_softmax(const PaParams &p, PpShared &sm, int u0, int u1, int 
             }
             named_sync(1, 256);
             if (sm.last) {
+#pragma unroll 1
                 for (int r = warp; r < s.rows; r += 8) {
                     auto at = [&](int c) { return p.partials + ((size_t)c * 2 + (c == c0 ? 1 : 0)) * kPpSlotFloats; };
                     float top = -INFINITY, l = 0.0f;
@@ -767,9 +768,9 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_attend_prompt_kernel(cons
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&sm.q_full[i], 4), mbar_init(&sm.turn[i], 4);
-            mbar_init(&sm.p_half[i], 4), mbar_init(&sm.p_full[i], 4);
-            mbar_init(&sm.s_full[i], 1), mbar_init(&sm.o_done[i], 1);
+            mbar_init(&sm.q_full[i], 4);
+            for (int h = 0; h < 2; ++h)
+                mbar_init(&sm.s_full[i][h], 1), mbar_init(&sm.p_full[i][h], 4), mbar_init(&sm.o_done[i][h], 1);
         }
         for (int i = 0; i < kPpStages; ++i) {
             mbar_init(&sm.k_full[i], 4), mbar_init(&sm.v_full[i], 4);
@@ -780,6 +781,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_attend_prompt_kernel(cons
         sm.abort = 0;
         fence_mbar_init();
     }
+#pragma unroll 1
     for (int b = warp; b < p.b.num_seqs; b += kPpThreads / 32) {
         const int n = pp_seq_units(p, pg_seq(p.b, p.c.page_size, b), lane) * p.c.kv_heads;
         if (lane == 0) sm.prefix[b + 1] = n;
@@ -788,6 +790,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_attend_prompt_kernel(cons
     if (warp == 0) {
         int before = 0;
         if (lane == 0) sm.prefix[0] = 0;
+#pragma unroll 1
         for (int b = 0; b < p.b.num_seqs; b += 32) {
             int incl = b + lane < p.b.num_seqs ? sm.prefix[b + lane + 1] : 0;
 #pragma unroll
