@@ -48,6 +48,13 @@ __device__ __forceinline__ uint32_t pg_e4m3x2_to_half2(uint32_t two) {
     return h;
 }
 
+// Four codes as two pairs of halves.
+__device__ __forceinline__ void pg_e4m3x4_to_half2(uint32_t four, uint32_t &lo, uint32_t &hi) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(four));
+}
+
 // A sequence's new tokens as the kernels see them (cut to the call's bounds): rows
 // [row0, row0 + count) of the call, at positions [pos0, pos0 + count), of a length of `len`.
 struct PgSeq {

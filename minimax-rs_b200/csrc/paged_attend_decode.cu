@@ -56,13 +56,6 @@ __device__ __forceinline__ uint32_t pd_transpose(uint32_t x) {
 __device__ __forceinline__ uint4 pd_lds(const uint8_t *tile, int row, int chunk) {
     return *reinterpret_cast<const uint4 *>(tile + row * kPgDim + ((chunk ^ (row & 7)) << 4));
 }
-// Four codes -> two f16 pairs.
-__device__ __forceinline__ void pd_cvt(uint32_t x, uint32_t &lo, uint32_t &hi) {
-    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
-        : "=r"(lo), "=r"(hi)
-        : "r"(x));
-}
-
 // An item's piece in this CTA's part of the list: sequence b, KV head h, steps [off, off + n) of the
 // item's nb.
 struct PdSeg {
@@ -325,8 +318,8 @@ struct PdKernel {
 #pragma unroll
                         for (int ks8 = 0; ks8 < 8; ++ks8) {
                             uint32_t a0, a1, a2, a3;
-                            pd_cvt(k0[ks8], a0, a2);
-                            pd_cvt(k1[ks8], a1, a3);
+                            pg_e4m3x4_to_half2(k0[ks8], a0, a2);
+                            pg_e4m3x4_to_half2(k1[ks8], a1, a3);
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt) {
                                 if constexpr (kQShared) {
@@ -397,8 +390,8 @@ struct PdKernel {
                         for (int half = 0; half < 2; ++half) {
                             const uint32_t sel = half ? 0x7362u : 0x5140u;
                             uint32_t a0, a1, a2, a3;
-                            pd_cvt(__byte_perm(x[0], x[1], sel), a0, a1);
-                            pd_cvt(__byte_perm(x[2], x[3], sel), a2, a3);
+                            pg_e4m3x4_to_half2(__byte_perm(x[0], x[1], sel), a0, a1);
+                            pg_e4m3x4_to_half2(__byte_perm(x[2], x[3], sel), a2, a3);
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt)
                                 pd_mma(o[nt][2 * w + half], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);

@@ -9,8 +9,8 @@
 //                    and sum, P (f16) back into S's columns, and the epilogue
 //   warps 8-11       K and V codes from global memory through registers (one tile ahead), e4m3 to
 //                    f16 (exact), into the operand layouts
-//   warp 12          issues S = Q K^T (both operands in shared memory) and O += P V (P in tensor
-//                    memory), kind::f16
+//   warps 12, 13     issue S = Q K^T (both operands in shared memory) and O += P V (P in tensor
+//                    memory), kind::f16, for tile 0, 1
 // Operand tiles are without swizzle: 16-byte pieces (8 columns of one row) with the eight rows of a
 // core matrix next to each other; the same form serves K (K-major) and V (its columns are the
 // product's N, so the tile is read MN-major).
@@ -53,7 +53,7 @@ struct PpShared {
     int prefix[kPaMaxSeqs + 1];
     uint64_t q_full[2], s_full[2][2], p_full[2][2], o_done[2][2];  // [row tile][half]
     uint64_t k_full[kPpStages], k_empty[kPpStages], v_full[kPpStages], v_empty[kPpStages], sc_full[kPpScales];
-    uint64_t mdone;
+    uint64_t mdone[2];
     uint32_t tmem;
     int abort, last;
 };
@@ -313,10 +313,8 @@ __device__ __forceinline__ void pp_store_tile(uint8_t *tile, const uint4 (&raw)[
         uint8_t *at = tile + 2 * chunk * kPpSlice + group * 128 + (lane & 7) * 16;
         const uint4 r = raw[it];
         uint4 a, b;
-        a.x = pg_e4m3x2_to_half2(r.x & 0xffffu), a.y = pg_e4m3x2_to_half2(r.x >> 16);
-        a.z = pg_e4m3x2_to_half2(r.y & 0xffffu), a.w = pg_e4m3x2_to_half2(r.y >> 16);
-        b.x = pg_e4m3x2_to_half2(r.z & 0xffffu), b.y = pg_e4m3x2_to_half2(r.z >> 16);
-        b.z = pg_e4m3x2_to_half2(r.w & 0xffffu), b.w = pg_e4m3x2_to_half2(r.w >> 16);
+        pg_e4m3x4_to_half2(r.x, a.x, a.y), pg_e4m3x4_to_half2(r.y, a.z, a.w);
+        pg_e4m3x4_to_half2(r.z, b.x, b.y), pg_e4m3x4_to_half2(r.w, b.z, b.w);
         if constexpr (kScaled) {
             const __half2 f = rel[it >> 2];
             auto times = [&](uint32_t &x) {
@@ -426,105 +424,100 @@ __device__ void pp_convert(const PaParams &p, PpShared &sm, int u0, int u1) {
     }
 }
 
-// ---- warp 12: the products -----------------------------------------------------------------------
+// ---- warps 12, 13: the products of row tile 0, 1 ------------------------------------------------
 // The whole warp walks the loops with values that the compiler can see to be uniform, and one
-// elected lane issues.  One warp issues for both row tiles, in turn: with a warp for each, the
-// products of the two interleave, both softmaxes get their scores at the same time, and then wait
-// for the products at the same time.
+// elected lane issues.
 __device__ __forceinline__ bool pp_elect() {
     uint32_t e;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
     return e != 0;
 }
 __device__ void pp_products(const PaParams &p, PpShared &sm, int u0, int u1) {
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, i = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5) - kPpMmaWarp, 0);
     const uint32_t tmem = __shfl_sync(0xffffffffu, sm.tmem, 0);
+    const uint32_t ts = tmem + kColS + 128 * i, to = tmem + kColO + 128 * i;
     // K-major operands: 16-byte K slices kPpSlice apart, 8-row groups 128 apart; V (MN-major): 8-key
     // groups 128 apart, 8-column groups kPpSlice apart
-    const uint32_t q0 = pp_desc_lo(smem_u32(sm.q[0]), kPpSlice);
+    const uint32_t q = pp_desc_lo(smem_u32(sm.q[i]), kPpSlice);
     const uint32_t k0 = pp_desc_lo(smem_u32(sm.k[0]), kPpSlice), v0 = pp_desc_lo(smem_u32(sm.v[0]), 128);
     // half h of a tile: its 64 keys' scores, columns [64 h, 64 h + 64) of the row tile's S
-    auto scores = [&](int i, int st, int h, bool last) {
-        const uint32_t a = q0 + i * (kPpTile >> 4), b = k0 + st * (kPpTile >> 4) + h * (8 * 128 >> 4);
+    auto scores = [&](int st, int h) {
+        const uint32_t b = k0 + st * (kPpTile >> 4) + h * (8 * 128 >> 4);
         if (pp_elect()) {
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-                pp_mma_ss(tmem + kColS + 128 * i + 64 * h, a + (k * 2 * kPpSlice >> 4), pp_desc_hi(128),
-                          b + (k * 2 * kPpSlice >> 4), pp_desc_hi(128), kPpIdescS, k > 0);
+                pp_mma_ss(ts + 64 * h, q + (k * 2 * kPpSlice >> 4), pp_desc_hi(128), b + (k * 2 * kPpSlice >> 4),
+                          pp_desc_hi(128), kPpIdescS, k > 0);
             tc_commit(&sm.s_full[i][h]);
-            if (h && last) tc_commit(&sm.k_empty[st]);
+            if (h) tc_commit(&sm.k_empty[st]);
         }
         __syncwarp();
     };
-    auto values = [&](int i, int st, int h, bool first, bool last) {
+    auto values = [&](int st, int h, bool first) {
         const uint32_t b = v0 + st * (kPpTile >> 4) + h * (4 * 256 >> 4);
         if (pp_elect()) {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                pp_mma_ts(tmem + kColO + 128 * i, tmem + kColS + 128 * i + 64 * h + 8 * k, b + (k * 256 >> 4),
-                          pp_desc_hi(kPpSlice), kPpIdescV, !(first && k == 0));
+                pp_mma_ts(to, ts + 64 * h + 8 * k, b + (k * 256 >> 4), pp_desc_hi(kPpSlice), kPpIdescV, !(first && k == 0));
             tc_commit(&sm.o_done[i][h]);
-            if (h && last) tc_commit(&sm.v_empty[st]);
+            if (h) tc_commit(&sm.v_empty[st]);
         }
         __syncwarp();
     };
     bool ok = true;
     auto wait = [&](uint64_t *bar, int use) {
         ok = ok && pp_wait_warp(bar, (uint32_t)use & 1, sm, p);
-        tc_fence_after();
         return ok;
     };
-    int tile = 0, pieces[2] = {0, 0}, used[2] = {0, 0};  // tiles so far; pieces, tiles of each row tile
+    auto test = [&](uint64_t *bar, int use) { return mbar_test_wait(bar, (uint32_t)use & 1); };
+    int tile = 0, pieces = 0, used = 0;  // tiles of the CTA so far; pieces and tiles of this row tile
 #pragma unroll 1
     for (int u = u0; ok && u < u1;) {
         PpSeg s;
         pp_seek(p, sm, u, u1, lane, s);
         const int n = __shfl_sync(0xffffffffu, s.n, 0);
-        const bool two = s.rows > 128;
-        wait(&sm.k_full[tile % kPpStages], tile / kPpStages);
+        if (i == 0 || s.rows > 128) {
+            wait(&sm.k_full[tile % kPpStages], tile / kPpStages);
+            wait(&sm.q_full[i], pieces);
+            tc_fence_after();
+            if (ok) scores(tile % kPpStages, 0);
+            if (ok) scores(tile % kPpStages, 1);
+            // A test of a barrier comes back late (it queues behind the softmaxes' exponentials), so all
+            // are asked together and only a phase found open is waited for.
 #pragma unroll 1
-        for (int x = 0; x < 4; ++x) {  // both halves of the first tile
-            const int i = x & 1, h = x >> 1;
-            if (i == 1 && !two) continue;
-            if (wait(&sm.q_full[i], pieces[i])) scores(i, tile % kPpStages, h, i == 1 || !two);
-        }
-        // A test of a barrier comes back late (it queues behind the softmaxes' exponentials), so each is
-        // asked ahead of its use and only a phase found open is waited for.
-        auto test = [&](uint64_t *bar, int use) { return mbar_test_wait(bar, (uint32_t)use & 1); };
-        bool p0 = false;
-#pragma unroll 1
-        for (int y = 0; ok && y < 2 * n; ++y) {
-            const int j = y >> 1, h = y & 1, at = tile + j, st = at % kPpStages, next = (at + 1) % kPpStages;
-            const bool more = j + 1 < n;
-            const bool v_in = test(&sm.v_full[st], at / kPpStages);
-            const bool k_in = !more || test(&sm.k_full[next], (at + 1) / kPpStages);
-            if (!p0) p0 = test(&sm.p_full[0][h], used[0] + j);
-            bool p1 = two && test(&sm.p_full[1][h], used[1] + j);
-            if (!__all_sync(0xffffffffu, v_in && k_in && p0)) {
-                wait(&sm.v_full[st], at / kPpStages);
-                if (more) wait(&sm.k_full[next], (at + 1) / kPpStages);
-                if (!wait(&sm.p_full[0][h], used[0] + j)) break;
+            for (int y = 0; ok && y < 2 * n; ++y) {
+                const int j = y >> 1, h = y & 1, at = tile + j, st = at % kPpStages, next = (at + 1) % kPpStages;
+                const bool more = j + 1 < n;
+                const bool v_in = test(&sm.v_full[st], at / kPpStages);
+                const bool k_in = !more || test(&sm.k_full[next], (at + 1) / kPpStages);
+                const bool p_in = test(&sm.p_full[i][h], used + j);
+                if (!__all_sync(0xffffffffu, v_in && k_in && p_in)) {
+                    wait(&sm.v_full[st], at / kPpStages);
+                    if (more) wait(&sm.k_full[next], (at + 1) / kPpStages);
+                    if (!wait(&sm.p_full[i][h], used + j)) break;
+                }
+                tc_fence_after();
+                values(st, h, y == 0);
+                // the products end in the order of their issue: P is read before the scores of the next
+                // tile's half overwrite it
+                if (more) scores(next, h);
             }
-            tc_fence_after();
-            values(0, st, h, y == 0, !two);
-            // the products end in the order of their issue: P is read before the scores of the next tile's
-            // half overwrite it
-            if (more) scores(0, next, h, !two);
-            p0 = y + 1 < 2 * n && test(&sm.p_full[0][h ^ 1], used[0] + ((y + 1) >> 1));
-            if (!two) continue;
-            if (!__all_sync(0xffffffffu, p1) && !wait(&sm.p_full[1][h], used[1] + j)) break;
-            tc_fence_after();
-            values(1, st, h, y == 0, true);
-            if (more) scores(1, next, h, true);
+            ++pieces;
+            used += n;
+        } else {  // an item of one row tile: this warp's share of the operands' release
+#pragma unroll 1
+            for (int j = 0; ok && j < n; ++j) {
+                const int at = tile + j, st = at % kPpStages;
+                if (wait(&sm.k_full[st], at / kPpStages) && lane == 0) mbar_arrive(&sm.k_empty[st]);
+                if (wait(&sm.v_full[st], at / kPpStages) && lane == 0) mbar_arrive(&sm.v_empty[st]);
+            }
         }
         tile += n;
-        ++pieces[0], used[0] += n;
-        if (two) ++pieces[1], used[1] += n;
         u += n;
     }
-    if (pp_elect()) tc_commit(&sm.mdone);  // every product has ended before the tensor memory goes
+    if (pp_elect()) tc_commit(&sm.mdone[i]);  // every product has ended before the tensor memory goes
     __syncwarp();
-    mbar_wait_bounded(&sm.mdone, 0, globaltimer_ns() + kPaTimeoutNs);
+    mbar_wait_bounded(&sm.mdone[i], 0, globaltimer_ns() + kPaTimeoutNs);
     __syncwarp();
 }
 
@@ -774,10 +767,10 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_attend_prompt_kernel(cons
         }
         for (int i = 0; i < kPpStages; ++i) {
             mbar_init(&sm.k_full[i], 4), mbar_init(&sm.v_full[i], 4);
-            mbar_init(&sm.k_empty[i], 1), mbar_init(&sm.v_empty[i], 1);
+            mbar_init(&sm.k_empty[i], 2), mbar_init(&sm.v_empty[i], 2);
         }
         for (int i = 0; i < kPpScales; ++i) mbar_init(&sm.sc_full[i], 4);
-        mbar_init(&sm.mdone, 1);
+        mbar_init(&sm.mdone[0], 1), mbar_init(&sm.mdone[1], 1);
         sm.abort = 0;
         fence_mbar_init();
     }
@@ -823,7 +816,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_attend_prompt_kernel(cons
         pp_convert(p, sm, u0, u1);
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-        if (warp == kPpMmaWarp) pp_products(p, sm, u0, u1);
+        if (warp < kPpMmaWarp + 2) pp_products(p, sm, u0, u1);
     }
     tc_fence_before();
     __syncthreads();
