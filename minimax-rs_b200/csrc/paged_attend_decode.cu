@@ -2,14 +2,18 @@
 //
 // Each K / V code is read once and used for all rows of its KV head, so the kernel is bound by HBM:
 // 256 bytes a position and head.  The products run on mma.sync with the operands turned round, S^T =
-// K Q^T and O^T += V^T P^T: the 16 positions of a step are the 16 rows of an instruction and eight
+// K Q^T and O^T += V^T P^T: 16 positions are the 16 rows of an instruction and eight
 // query rows its columns, so that six query heads waste two columns of eight instead of ten rows
 // of sixteen.  Which code goes to which contraction index is free as long as both operands agree,
 // so a lane takes 32 consecutive codes of a key row (two 16-byte reads) and 16 of a value row, and
 // turns them into f16 pairs in registers (e4m3 to f16 is exact).  P^T comes from S^T's accumulators
 // by a transposing move of 8x8 tiles.
 //
-// Work: the steps of 16 positions of all sequences and KV heads form one list, of which every CTA
+// The running maximum of a column moves only when a score passes it by more than 2^8 (P then still
+// fits f16), found by one vote over the step's scores: the usual step neither reduces a maximum over
+// lanes nor touches O.
+//
+// Work: the steps of 32 positions of all sequences and KV heads form one list, of which every CTA
 // (one per SM) takes an equal, contiguous part; a CTA's eight warps take its steps in turn, each
 // with a ring of TMA copies of its own, its own running maximum and sum, and no barrier until the end
 // of a (sequence, head).  Where that end lies in another CTA, the CTAs' partial results go through
@@ -24,17 +28,18 @@ namespace {
 
 constexpr int kPdWarps = 8;
 constexpr int kPdThreads = 32 * kPdWarps;
-constexpr int kPdStep = 16;                       // positions of a step
+constexpr int kPdStep = 32;                       // positions of a step: two groups of 16, each in one page
 constexpr int kPdTile = kPdStep * kPgDim;         // bytes of its keys (or values)
-constexpr int kPdStages = 5;
+constexpr int kPdStages = 3;
+constexpr float kPdLazy = 8.0f;                   // log2 of how far P may exceed 1
 constexpr int kPdRowFloats = kPgDim + 4;          // a row of the merge buffer
 
 struct PdShared {
     uint8_t ring[kPdWarps][kPdStages][2][kPdTile];  // 1024-byte aligned tiles (swizzled)
-    float o[kPdWarps][8][kPdRowFloats];             // one eight-row group of every warp's sums
+    float o[kPdWarps / 2][8][kPdRowFloats];         // one eight-row group of half the warps' sums
     uint32_t q[8][4][32][2];                        // NT = 3, 4: the queries' fragments
     float m[kPdWarps][32], l[kPdWarps][32];
-    float meta[kPdWarps][kPdStages][2];             // scales of the stage's page (k < 0: nothing there)
+    float4 meta[kPdWarps][kPdStages];               // k, v scale of the stage's two groups (k < 0: nothing there)
     uint64_t full[kPdWarps][kPdStages];
     int prefix[kPaMaxSeqs + 1];
     int scan[kPdWarps];
@@ -68,6 +73,7 @@ template <int NT, typename T>
 struct PdKernel {
     static constexpr int kRows = 8 * NT;
     static constexpr bool kQShared = NT > 2;
+    static constexpr int kE = NT > 2 ? 1 : 2;
 
     static __device__ int item_steps(const PaParams &p, int b, PgSeq &seq, PaSpan<kPdStep> &span) {
         seq = pg_seq(p.b, p.c.page_size, b);
@@ -181,8 +187,8 @@ struct PdKernel {
         // ---- the copies: a cursor over this warp's steps, up to kPdStages ahead of the products
         PdSeg in;
         int in_u = u0, in_i = warp, in_base = 0, issued = 0;
-        int pid = -1;
-        float ks = 0.0f, vs = 0.0f;
+        int row = -1;
+        float ks = -1.0f, vs = 0.0f;
         bool in_open = false, in_done = false;
         auto issue = [&]() {
             while (!in_done) {
@@ -198,36 +204,40 @@ struct PdKernel {
                 in_done = in_u >= u1;
             }
             if (in_done) return;
-            const int batch = (in_i - warp) / (32 * kPdWarps);
-            if (batch != in_base) {  // the pages and scales of this warp's next 32 steps, one a lane
-                in_base = batch;
-                const int i = warp + kPdWarps * (batch * 32 + lane);
-                pid = -1;
+            const int at = in_i / kPdWarps;  // this warp's how-manieth step of the piece
+            if (at >> 4 != in_base) {        // the pages and scales of its next 16 steps' groups, one a lane
+                in_base = at >> 4;
+                const int i = warp + kPdWarps * ((at & ~15) + (lane >> 1));
+                row = -1;
+                ks = -1.0f, vs = 0.0f;
                 if (i < in.n) {
-                    const int j = in.span.step(in.off + i) * kPdStep;
+                    const int j = in.span.step(in.off + i) * kPdStep + 16 * (lane & 1);
+                    int pid = -1;
                     if (j < in.seq.len) pid = p.b.page_table[(long)in.b * p.b.table_stride + j / p.c.page_size];
-                    if (pid >= p.c.num_pages) pid = -1;
-                }
-                if (pid >= 0) {
-                    ks = p.c.k_scale[(long)pid * p.c.kv_heads + in.h];
-                    vs = p.c.v_scale[(long)pid * p.c.kv_heads + in.h];
+                    if (pid >= 0 && pid < p.c.num_pages) {
+                        const int ph = pid * p.c.kv_heads + in.h;
+                        row = ph * p.c.page_size + (j & (p.c.page_size - 1));
+                        ks = p.c.k_scale[ph];
+                        vs = p.c.v_scale[ph];
+                    }
                 }
             }
-            const int src = (in_i - warp) / kPdWarps & 31;
-            const int page = __shfl_sync(0xffffffffu, pid, src);
-            const float k1 = __shfl_sync(0xffffffffu, ks, src), v1 = __shfl_sync(0xffffffffu, vs, src);
-            if (lane == 0) {
-                const int st = issued % kPdStages;
-                sm.meta[warp][st][0] = page < 0 ? -1.0f : k1;
-                sm.meta[warp][st][1] = v1;
-                if (page < 0) {
-                    mbar_arrive(&sm.full[warp][st]);
-                } else {
-                    const int j = in.span.step(in.off + in_i) * kPdStep;
-                    const int row = (page * p.c.kv_heads + in.h) * p.c.page_size + j % p.c.page_size;
-                    mbar_arrive_expect_tx(&sm.full[warp][st], 2 * kPdTile);
-                    pa_tma_2d(sm.ring[warp][st][0], kmap, 0, row, &sm.full[warp][st]);
-                    pa_tma_2d(sm.ring[warp][st][1], vmap, 0, row, &sm.full[warp][st]);
+            const int st = issued % kPdStages;
+            if ((lane >> 1) == (at & 15)) {  // the two lanes that know the step's groups
+                const uint32_t pair = 3u << (lane & ~1);
+                const int other = __shfl_xor_sync(pair, row, 1);
+                reinterpret_cast<float2 *>(&sm.meta[warp][st])[lane & 1] = make_float2(ks, vs);
+                uint64_t *bar = &sm.full[warp][st];
+                if (!(lane & 1)) {
+                    const int n = (row >= 0) + (other >= 0);
+                    if (n) mbar_arrive_expect_tx(bar, n * kPdTile);
+                    else mbar_arrive(bar);
+                }
+                __syncwarp(pair);
+                if (row >= 0) {
+                    const int half = (lane & 1) * (kPdTile / 2);
+                    pa_tma_2d(sm.ring[warp][st][0] + half, kmap, 0, row, bar);
+                    pa_tma_2d(sm.ring[warp][st][1] + half, vmap, 0, row, bar);
                 }
             }
             ++issued;
@@ -298,20 +308,34 @@ struct PdKernel {
                     atomicExch(p.status, (uint32_t)MMRS_ERR_TIMEOUT);
                 }
                 __syncwarp();
-                const float ksc = sm.meta[warp][st][0], vsc = sm.meta[warp][st][1];
-                if (ksc >= 0.0f || ksc != ksc) {
+                const float4 scales = sm.meta[warp][st];
+                const float ksc[2] = {scales.x, scales.z}, vsc[2] = {scales.y, scales.w};
+                const bool in0 = !(ksc[0] < 0.0f), in1 = !(ksc[1] < 0.0f);
+                if (in0 || in1) {
                     const int j0 = s.span.step(s.off + i) * kPdStep;
                     const uint8_t *kt = sm.ring[warp][st][0], *vt = sm.ring[warp][st][1];
-                    float sc[NT][4];
+                    const bool whole = in0 && in1 && j0 + kPdStep - 1 <= pos_lo &&
+                                       (p.window <= 0 || pos_hi - j0 < p.window || j0 + kPdStep <= p.sinks);
+                    // kE groups at a time: both, where the registers allow it
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+                    for (int e0 = 0; e0 < 2; e0 += kE) {
+                    float sc[kE][NT][4];
+                    bool over = false;
+                    auto largest = [&](int nt, int c) {
+                        float mx = fmaxf(sc[0][nt][c], sc[0][nt][c + 2]);
+                        if constexpr (kE == 2) mx = fmaxf(mx, fmaxf(sc[kE - 1][nt][c], sc[kE - 1][nt][c + 2]));
+                        return mx;
+                    };
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) sc[nt][c] = 0.0f;
-                    {
+                    for (int e = 0; e < kE; ++e) {
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) sc[e][nt][c] = 0.0f;
                         uint32_t k0[8], k1[8];
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
-                            const uint4 x = pd_lds(kt, g, 2 * t + c), y = pd_lds(kt, g + 8, 2 * t + c);
+                            const uint4 x = pd_lds(kt, 16 * (e0 + e) + g, 2 * t + c), y = pd_lds(kt, 16 * (e0 + e) + g + 8, 2 * t + c);
                             k0[4 * c] = x.x, k0[4 * c + 1] = x.y, k0[4 * c + 2] = x.z, k0[4 * c + 3] = x.w;
                             k1[4 * c] = y.x, k1[4 * c + 1] = y.y, k1[4 * c + 2] = y.z, k1[4 * c + 3] = y.w;
                         }
@@ -324,78 +348,104 @@ struct PdKernel {
                             for (int nt = 0; nt < NT; ++nt) {
                                 if constexpr (kQShared) {
                                     const uint2 b = *reinterpret_cast<const uint2 *>(sm.q[ks8][nt][lane]);
-                                    pd_mma(sc[nt], a0, a1, a2, a3, b.x, b.y);
+                                    pd_mma(sc[e][nt], a0, a1, a2, a3, b.x, b.y);
                                 } else {
-                                    pd_mma(sc[nt], a0, a1, a2, a3, qf[nt][2 * ks8], qf[nt][2 * ks8 + 1]);
+                                    pd_mma(sc[e][nt], a0, a1, a2, a3, qf[nt][2 * ks8], qf[nt][2 * ks8 + 1]);
                                 }
                             }
                         }
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int c = 0; c < 2; ++c) {
+                                const float f = qs[nt][c] * ksc[e0 + e];
+                                sc[e][nt][c] *= f, sc[e][nt][c + 2] *= f;
+                            }
                     }
-                    const bool whole = j0 + kPdStep - 1 <= pos_lo &&
-                                       (p.window <= 0 || pos_hi - j0 < p.window || j0 + kPdStep <= p.sinks);
+                    if (!whole) {
+#pragma unroll
+                        for (int e = 0; e < kE; ++e)
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int c = 0; c < 4; ++c)
+                                    if (!(e0 + e ? in1 : in0) ||
+                                        !pa_sees(j0 + 16 * (e0 + e) + g + (c >> 1) * 8, pos[nt][c & 1], p.window, p.sinks))
+                                        sc[e][nt][c] = -INFINITY;
+                    }
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            sc[nt][c] *= qs[nt][c & 1] * ksc;
-                            if (!whole && !pa_sees(j0 + g + (c >> 1) * 8, pos[nt][c & 1], p.window, p.sinks))
-                                sc[nt][c] = -INFINITY;
-                        }
+                        for (int c = 0; c < 2; ++c)
+                            over = over || largest(nt, c) > m[nt][c] + kPdLazy;
                     // the values' scale: probabilities are stored relative to the largest seen
-                    float vfac = 1.0f;
-                    if (vsc > vref) {
-                        vfac = vref / vsc;
-                        vref = vsc;
+                    const float vtop = kE == 2 ? fmaxf(vsc[0], vsc[1]) : vsc[e0];
+                    if (vtop > vref || __any_sync(0xffffffffu, over)) {
+                        const float vfac = vtop > vref ? vref / vtop : 1.0f;
+                        vref = fmaxf(vref, vtop);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int c = 0; c < 2; ++c) {
+                                float mx = largest(nt, c);
+                                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                                mx = fmaxf(mx, m[nt][c]);
+                                const float fac = mx == -INFINITY ? 1.0f : pa_exp2(m[nt][c] - mx), of = fac * vfac;
+                                m[nt][c] = mx;
+                                l[nt][c] *= fac;
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) o[nt][j][c] *= of, o[nt][j][c + 2] *= of;
+                            }
                     }
-                    const float vr = vref > 0.0f ? vsc / vref : 0.0f;
-                    uint32_t pb[NT][2];
+                    const float vinv = vref > 0.0f ? 1.0f / vref : 0.0f;
+                    uint32_t pb[kE][NT][2];
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        float p4[4];
+                    for (int e = 0; e < kE; ++e) {
+                        const float vr = vsc[e0 + e] * vinv;
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            float mx = fmaxf(sc[nt][c], sc[nt][c + 2]);
-                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                            mx = fmaxf(mx, m[nt][c]);
-                            const float base = mx == -INFINITY ? 0.0f : mx;
-                            const float fac = pa_exp2(m[nt][c] - base);
-                            m[nt][c] = mx;
-                            p4[c] = pa_exp2(sc[nt][c] - base);
-                            p4[c + 2] = pa_exp2(sc[nt][c + 2] - base);
-                            l[nt][c] = l[nt][c] * fac + p4[c] + p4[c + 2];
-                            const float of = fac * vfac;
+                        for (int nt = 0; nt < NT; ++nt) {
+                            float p4[4];
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) o[nt][j][c] *= of, o[nt][j][c + 2] *= of;
+                            for (int c = 0; c < 2; ++c) {
+                                const float base = m[nt][c] == -INFINITY ? 0.0f : m[nt][c];
+                                p4[c] = pa_exp2(sc[e][nt][c] - base);
+                                p4[c + 2] = pa_exp2(sc[e][nt][c + 2] - base);
+                                l[nt][c] += p4[c] + p4[c + 2];
+                            }
+                            pb[e][nt][0] = pd_transpose(pg_pack2(p4[0] * vr, p4[1] * vr, (const __half *)nullptr));
+                            pb[e][nt][1] = pd_transpose(pg_pack2(p4[2] * vr, p4[3] * vr, (const __half *)nullptr));
                         }
-                        pb[nt][0] = pd_transpose(pg_pack2(p4[0] * vr, p4[1] * vr, (const __half *)nullptr));
-                        pb[nt][1] = pd_transpose(pg_pack2(p4[2] * vr, p4[3] * vr, (const __half *)nullptr));
-                    }
-                    uint4 v4[4];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const int row = 2 * t + (c & 1) + (c >> 1) * 8;
-                        v4[c] = pd_lds(vt, row, g);
-                        // slots past the sequence's end may hold anything
-                        if (!whole && j0 + row >= s.seq.len) v4[c] = make_uint4(0u, 0u, 0u, 0u);
                     }
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const uint32_t x[4] = {reinterpret_cast<const uint32_t *>(&v4[0])[w],
-                                               reinterpret_cast<const uint32_t *>(&v4[1])[w],
-                                               reinterpret_cast<const uint32_t *>(&v4[2])[w],
-                                               reinterpret_cast<const uint32_t *>(&v4[3])[w]};
+                    for (int e = 0; e < kE; ++e) {
+                        uint4 v4[4];
 #pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            const uint32_t sel = half ? 0x7362u : 0x5140u;
-                            uint32_t a0, a1, a2, a3;
-                            pg_e4m3x4_to_half2(__byte_perm(x[0], x[1], sel), a0, a1);
-                            pg_e4m3x4_to_half2(__byte_perm(x[2], x[3], sel), a2, a3);
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt)
-                                pd_mma(o[nt][2 * w + half], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+                        for (int c = 0; c < 4; ++c) {
+                            const int r = 2 * t + (c & 1) + (c >> 1) * 8;
+                            v4[c] = pd_lds(vt, 16 * (e0 + e) + r, g);
+                            // slots past the sequence's end may hold anything
+                            if (!whole && (!(e0 + e ? in1 : in0) || j0 + 16 * (e0 + e) + r >= s.seq.len)) v4[c] = make_uint4(0u, 0u, 0u, 0u);
                         }
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            const uint32_t x[4] = {reinterpret_cast<const uint32_t *>(&v4[0])[w],
+                                                   reinterpret_cast<const uint32_t *>(&v4[1])[w],
+                                                   reinterpret_cast<const uint32_t *>(&v4[2])[w],
+                                                   reinterpret_cast<const uint32_t *>(&v4[3])[w]};
+#pragma unroll
+                            for (int half = 0; half < 2; ++half) {
+                                const uint32_t sel = half ? 0x7362u : 0x5140u;
+                                uint32_t a0, a1, a2, a3;
+                                pg_e4m3x4_to_half2(__byte_perm(x[0], x[1], sel), a0, a1);
+                                pg_e4m3x4_to_half2(__byte_perm(x[2], x[3], sel), a2, a3);
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt)
+                                    pd_mma(o[nt][2 * w + half], a0, a1, a2, a3, pb[e][nt][0], pb[e][nt][1]);
+                            }
+                        }
+                    }
                     }
                 }
                 __syncwarp();
@@ -416,18 +466,37 @@ struct PdKernel {
             __syncthreads();
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
+                // every warp's sums to the common maximum; the upper four warps' into the lower's
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const int r = nt * 8 + 2 * t + c;
                     float top = -INFINITY;
 #pragma unroll
                     for (int w = 0; w < kPdWarps; ++w) top = fmaxf(top, sm.m[w][r]);
-                    const float f = top == -INFINITY ? 1.0f : pa_exp2(m[nt][c] - top);
+                    const float f = (top == -INFINITY ? 1.0f : pa_exp2(m[nt][c] - top)) * vref;
 #pragma unroll
-                    for (int j = 0; j < 8; j += 2)
-                        *reinterpret_cast<float4 *>(&sm.o[warp][2 * t + c][16 * g + 2 * j]) =
-                            make_float4(o[nt][j][c] * f * vref, o[nt][j][c + 2] * f * vref, o[nt][j + 1][c] * f * vref,
-                                        o[nt][j + 1][c + 2] * f * vref);
+                    for (int j = 0; j < 8; ++j) o[nt][j][c] *= f, o[nt][j][c + 2] *= f;
+                }
+                auto sums = [&](int c, int j) {
+                    return reinterpret_cast<float4 *>(&sm.o[warp % (kPdWarps / 2)][2 * t + c][16 * g + 2 * j]);
+                };
+                if (warp >= kPdWarps / 2) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int j = 0; j < 8; j += 2)
+                            *sums(c, j) = make_float4(o[nt][j][c], o[nt][j][c + 2], o[nt][j + 1][c], o[nt][j + 1][c + 2]);
+                }
+                __syncthreads();
+                if (warp < kPdWarps / 2) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int j = 0; j < 8; j += 2) {
+                            const float4 x = *sums(c, j);
+                            *sums(c, j) = make_float4(o[nt][j][c] + x.x, o[nt][j][c + 2] + x.y, o[nt][j + 1][c] + x.z,
+                                                      o[nt][j + 1][c + 2] + x.w);
+                        }
                 }
                 __syncthreads();
                 {
@@ -439,6 +508,9 @@ struct PdKernel {
 #pragma unroll
                     for (int w = 0; w < kPdWarps; ++w) {
                         sum_l += sm.l[w][r] * (top == -INFINITY ? 1.0f : pa_exp2(sm.m[w][r] - top));
+                    }
+#pragma unroll
+                    for (int w = 0; w < kPdWarps / 2; ++w) {
                         const float4 x = *reinterpret_cast<const float4 *>(&sm.o[w][warp][4 * lane]);
                         acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
                     }
