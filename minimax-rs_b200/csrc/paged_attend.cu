@@ -104,11 +104,12 @@ extern "C" int mmrs_paged_attend(const MmrsPagedCache *cache, const MmrsPagedBat
     // a sequence has no more rows than the call; work units are counted with 32 bits
     const long max_q = batch->max_q < batch->total_q ? batch->max_q : batch->total_q;
     if (max_q * p.group <= kPaDecodeRows) {
-        if ((long)batch->num_seqs * cache->kv_heads * (batch->max_len / 16 + 1) > 0x3fffffffL) return MMRS_ERR_UNSUPPORTED;
+        if ((long)batch->num_seqs * cache->kv_heads * (batch->max_len / 16 + 32) > 0x3fffffffL) return MMRS_ERR_UNSUPPORTED;
         p.b.max_q = (int)max_q;
         CUtensorMap kmap, vmap;
-        int mc = pa_make_map(&kmap, cache->k, *cache, 16);
-        if (mc == MMRS_OK) mc = pa_make_map(&vmap, cache->v, *cache, 16);
+        const int rows = cache->page_size < 32 ? 16 : 32;
+        int mc = pa_make_map(&kmap, cache->k, *cache, rows);
+        if (mc == MMRS_OK) mc = pa_make_map(&vmap, cache->v, *cache, rows);
         return mc != MMRS_OK ? mc : pa_launch_decode(p, kmap, vmap, type, (cudaStream_t)stream);
     }
     if (((long)batch->total_q * p.group / 256 + batch->num_seqs) * cache->kv_heads * (batch->max_len / 128 + 1) > 0x3fffffffL)

@@ -14,7 +14,7 @@
 // lanes nor touches O.
 //
 // Work: the steps of 32 positions of all sequences and KV heads form one list, of which every CTA
-// (one per SM) takes an equal, contiguous part; a CTA's eight warps take its steps in turn, each
+// (one per SM) takes an equal, contiguous part; a CTA's warps take its steps in turn, each
 // with a ring of TMA copies of its own, its own running maximum and sum, and no barrier until the end
 // of a (sequence, head).  Where that end lies in another CTA, the CTAs' partial results go through
 // the workspace and the last to arrive joins them in order.
@@ -26,18 +26,25 @@
 namespace mmrs {
 namespace {
 
-constexpr int kPdWarps = 8;
-constexpr int kPdThreads = 32 * kPdWarps;
 constexpr int kPdStep = 32;                       // positions of a step: two groups of 16, each in one page
 constexpr int kPdTile = kPdStep * kPgDim;         // bytes of its keys (or values)
-constexpr int kPdStages = 3;
 constexpr float kPdLazy = 8.0f;                   // log2 of how far P may exceed 1
+constexpr float kPdNone = -1e30f;                 // below every score
 constexpr int kPdRowFloats = kPgDim + 4;          // a row of the merge buffer
 
+constexpr int kPdWarps = 8;
+constexpr int kPdThreads = 32 * kPdWarps;
+constexpr int kPdStages = 2;
+// What beginning and ending a (sequence, head) costs a block, in steps: the list is cut into equal
+// parts with that much added to each item, else blocks over many short sequences end last (at 64
+// sequences of 1000 to 8000 positions the last block took 1.4 times the average).
+constexpr int kPdItemCost = 24;
+
+template <int NT>
 struct PdShared {
     uint8_t ring[kPdWarps][kPdStages][2][kPdTile];  // 1024-byte aligned tiles (swizzled)
-    float o[kPdWarps / 2][8][kPdRowFloats];         // one eight-row group of half the warps' sums
-    uint32_t q[8][4][32][2];                        // NT = 3, 4: the queries' fragments
+    float o[kPdWarps / 2][8 * NT][kPdRowFloats];    // half the warps' sums
+    uint32_t q[NT > 2 ? 8 : 1][4][32][2];           // NT = 3, 4: the queries' fragments
     float m[kPdWarps][32], l[kPdWarps][32];
     float4 meta[kPdWarps][kPdStages];               // k, v scale of the stage's two groups (k < 0: nothing there)
     uint64_t full[kPdWarps][kPdStages];
@@ -62,27 +69,27 @@ __device__ __forceinline__ uint4 pd_lds(const uint8_t *tile, int row, int chunk)
     return *reinterpret_cast<const uint4 *>(tile + row * kPgDim + ((chunk ^ (row & 7)) << 4));
 }
 // An item's piece in this CTA's part of the list: sequence b, KV head h, steps [off, off + n) of the
-// item's nb.
+// item's nb; the item's first step is unit `first` of the list, after its cost.
 struct PdSeg {
-    int b, h, off, n, nb;
+    int b, h, off, n, nb, first;
     PgSeq seq;
     PaSpan<kPdStep> span;
 };
 
 template <int NT, typename T>
 struct PdKernel {
-    static constexpr int kRows = 8 * NT;
+    static constexpr int kRows = 8 * NT, kSeqs = kPaMaxSeqs / kPdThreads;  // (sequences a thread counts)
     static constexpr bool kQShared = NT > 2;
-    static constexpr int kE = NT > 2 ? 1 : 2;
+    static constexpr int kE = NT <= 2 ? 2 : 1;
 
     static __device__ int item_steps(const PaParams &p, int b, PgSeq &seq, PaSpan<kPdStep> &span) {
         seq = pg_seq(p.b, p.c.page_size, b);
         span = pa_span<kPdStep>(max(seq.pos0, 0), seq.len - 1, p.window, p.sinks);
-        return seq.count > 0 ? max(span.n, 1) : 0;  // rows that see nothing are written too
+        return seq.count > 0 ? max(span.n, 1) + kPdItemCost : 0;  // rows that see nothing are written too
     }
 
     // The piece that starts at unit u (< end, the CTA's end; `total` units in all).
-    static __device__ void seek(const PaParams &p, const PdShared &sm, int u, int end, PdSeg &s) {
+    static __device__ void seek(const PaParams &p, const PdShared<NT> &sm, int u, int end, PdSeg &s) {
         int lo = 0, hi = p.b.num_seqs;  // the last sequence with prefix <= u
         while (hi - lo > 1) {
             const int mid = (lo + hi) / 2;
@@ -90,11 +97,12 @@ struct PdKernel {
             else hi = mid;
         }
         s.b = lo;
-        s.nb = item_steps(p, lo, s.seq, s.span);
-        const int at = u - sm.prefix[lo];
-        s.h = at / s.nb;
-        s.off = at - s.h * s.nb;
-        s.n = min(s.nb - s.off, end - u);
+        const int units = item_steps(p, lo, s.seq, s.span), at = u - sm.prefix[lo];
+        s.nb = units - kPdItemCost;
+        s.h = at / units;
+        s.first = sm.prefix[lo] + s.h * units + kPdItemCost;
+        s.off = max(u - s.first, 0);
+        s.n = min(s.nb, end - s.first) - s.off;  // not positive: only the item's cost lies before `end`
     }
 
     static __device__ void load_q(const PaParams &p, const PdSeg &s, int lane, int nt, uint32_t (&f)[16], float &factor) {
@@ -143,7 +151,7 @@ struct PdKernel {
         if (p.lse && lane == 0) p.lse[at] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kPaLn2;
     }
 
-    static __device__ void run(const PaParams &p, const CUtensorMap *kmap, const CUtensorMap *vmap, PdShared &sm) {
+    static __device__ void run(const PaParams &p, const CUtensorMap *kmap, const CUtensorMap *vmap, PdShared<NT> &sm) {
         const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
         const uint64_t deadline = globaltimer_ns() + kPaTimeoutNs;
         if (lane == 0) {
@@ -151,10 +159,10 @@ struct PdKernel {
             fence_mbar_init();
         }
         // prefix sums of the sequences' units: each thread takes four consecutive sequences
-        int mine[kPaMaxSeqs / kPdThreads], sum = 0;
+        int mine[kSeqs], sum = 0;
 #pragma unroll
-        for (int i = 0; i < kPaMaxSeqs / kPdThreads; ++i) {
-            const int b = tid * (kPaMaxSeqs / kPdThreads) + i;
+        for (int i = 0; i < kSeqs; ++i) {
+            const int b = tid * (kSeqs) + i;
             PgSeq seq;
             PaSpan<kPdStep> span;
             mine[i] = b < p.b.num_seqs ? item_steps(p, b, seq, span) * p.c.kv_heads : 0;
@@ -175,8 +183,8 @@ struct PdKernel {
             total += sm.scan[w];
         }
 #pragma unroll
-        for (int i = 0; i < kPaMaxSeqs / kPdThreads; ++i) {
-            sm.prefix[tid * (kPaMaxSeqs / kPdThreads) + i] = before;
+        for (int i = 0; i < kSeqs; ++i) {
+            sm.prefix[tid * kSeqs + i] = before;
             before += mine[i];
         }
         __syncthreads();
@@ -199,7 +207,7 @@ struct PdKernel {
                     in_open = true;
                 }
                 if (in_i < in.n) break;
-                in_u += in.n;
+                in_u = in.first + in.nb;
                 in_open = false;
                 in_done = in_u >= u1;
             }
@@ -213,7 +221,9 @@ struct PdKernel {
                 if (i < in.n) {
                     const int j = in.span.step(in.off + i) * kPdStep + 16 * (lane & 1);
                     int pid = -1;
-                    if (j < in.seq.len) pid = p.b.page_table[(long)in.b * p.b.table_stride + j / p.c.page_size];
+                    // (a page that holds both groups counts for both, wherever the sequence ends in it)
+                    if ((p.c.page_size == 16 ? j : j & ~31) < in.seq.len)
+                        pid = p.b.page_table[(long)in.b * p.b.table_stride + j / p.c.page_size];
                     if (pid >= 0 && pid < p.c.num_pages) {
                         const int ph = pid * p.c.kv_heads + in.h;
                         row = ph * p.c.page_size + (j & (p.c.page_size - 1));
@@ -234,7 +244,8 @@ struct PdKernel {
                     else mbar_arrive(bar);
                 }
                 __syncwarp(pair);
-                if (row >= 0) {
+                // pages of 32 positions and more hold both groups: one copy each of keys and values
+                if (row >= 0 && (p.c.page_size == 16 || !(lane & 1))) {
                     const int half = (lane & 1) * (kPdTile / 2);
                     pa_tma_2d(sm.ring[warp][st][0] + half, kmap, 0, row, bar);
                     pa_tma_2d(sm.ring[warp][st][1] + half, vmap, 0, row, bar);
@@ -250,6 +261,8 @@ struct PdKernel {
         for (int u = u0; u < u1;) {
             PdSeg s;
             seek(p, sm, u, u1, s);
+            u = s.first + s.nb;
+            if (s.n <= 0) continue;
             const int rows = min(s.seq.count * p.group, kRows);
             uint32_t qf[kQShared ? 1 : NT][16];
             float qs[NT][2];  // the score's factor for this lane's two columns
@@ -260,7 +273,11 @@ struct PdKernel {
                 if (!kQShared || warp == nt) {
                     uint32_t f[16];
                     load_q(p, s, lane, nt, f, up);
-                    up = to_f16(f);
+                    up = to_f16(f) * fabsf(p.scale_log2);
+                    if (p.scale_log2 < 0.0f) {  // the columns' factors stay >= 0
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) f[i] ^= 0x80008000u;
+                    }
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         if constexpr (kQShared) sm.q[i / 2][nt][lane][i & 1] = f[i];
@@ -270,8 +287,8 @@ struct PdKernel {
                         if (t == 0) sm.m[0][nt * 8 + g] = up;
                 }
                 if constexpr (!kQShared) {
-                    qs[nt][0] = __shfl_sync(0xffffffffu, up, 8 * t) * p.scale_log2;
-                    qs[nt][1] = __shfl_sync(0xffffffffu, up, 8 * t + 4) * p.scale_log2;
+                    qs[nt][0] = __shfl_sync(0xffffffffu, up, 8 * t);
+                    qs[nt][1] = __shfl_sync(0xffffffffu, up, 8 * t + 4);
                 }
             }
             if constexpr (kQShared) {
@@ -279,7 +296,7 @@ struct PdKernel {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) qs[nt][c] = sm.m[0][nt * 8 + 2 * t + c] * p.scale_log2;
+                    for (int c = 0; c < 2; ++c) qs[nt][c] = sm.m[0][nt * 8 + 2 * t + c];
                 __syncthreads();
             }
 #pragma unroll
@@ -290,12 +307,12 @@ struct PdKernel {
                     pos[nt][c] = r < rows ? s.seq.pos0 + r / p.group : -1;
                 }
             const int pos_lo = s.seq.pos0, pos_hi = s.seq.len - 1;
-            float m[NT][2], l[NT][2], o[NT][8][4];
+            float m[NT][2], l[NT][2], o[NT][8][4];  // per column; the maximum kPdNone before the first score
             float vref = 0.0f;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                for (int c = 0; c < 2; ++c) m[nt][c] = -INFINITY, l[nt][c] = 0.0f;
+                for (int c = 0; c < 2; ++c) m[nt][c] = kPdNone, l[nt][c] = 0.0f;
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
 #pragma unroll
@@ -321,9 +338,12 @@ struct PdKernel {
                     for (int e0 = 0; e0 < 2; e0 += kE) {
                     float sc[kE][NT][4];
                     bool over = false;
+                    // a column's factor: never 0, so that a masked score's -infinity stays one
+                    auto factor = [&](int e, int nt, int c) { return fmaxf(qs[nt][c] * ksc[e0 + e], 1e-35f); };
                     auto largest = [&](int nt, int c) {
-                        float mx = fmaxf(sc[0][nt][c], sc[0][nt][c + 2]);
-                        if constexpr (kE == 2) mx = fmaxf(mx, fmaxf(sc[kE - 1][nt][c], sc[kE - 1][nt][c + 2]));
+                        float mx = fmaxf(sc[0][nt][c], sc[0][nt][c + 2]) * factor(0, nt, c);
+                        if constexpr (kE == 2)
+                            mx = fmaxf(mx, fmaxf(sc[kE - 1][nt][c], sc[kE - 1][nt][c + 2]) * factor(kE - 1, nt, c));
                         return mx;
                     };
 #pragma unroll
@@ -354,13 +374,6 @@ struct PdKernel {
                                 }
                             }
                         }
-#pragma unroll
-                        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                            for (int c = 0; c < 2; ++c) {
-                                const float f = qs[nt][c] * ksc[e0 + e];
-                                sc[e][nt][c] *= f, sc[e][nt][c + 2] *= f;
-                            }
                     }
                     if (!whole) {
 #pragma unroll
@@ -392,7 +405,7 @@ struct PdKernel {
                                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
                                 mx = fmaxf(mx, m[nt][c]);
-                                const float fac = mx == -INFINITY ? 1.0f : pa_exp2(m[nt][c] - mx), of = fac * vfac;
+                                const float fac = pa_exp2(m[nt][c] - mx), of = fac * vfac;
                                 m[nt][c] = mx;
                                 l[nt][c] *= fac;
 #pragma unroll
@@ -403,19 +416,24 @@ struct PdKernel {
                     uint32_t pb[kE][NT][2];
 #pragma unroll
                     for (int e = 0; e < kE; ++e) {
-                        const float vr = vsc[e0 + e] * vinv;
+                        const __half2 vr = __float2half2_rn(vsc[e0 + e] * vinv);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
                             float p4[4];
 #pragma unroll
                             for (int c = 0; c < 2; ++c) {
-                                const float base = m[nt][c] == -INFINITY ? 0.0f : m[nt][c];
-                                p4[c] = pa_exp2(sc[e][nt][c] - base);
-                                p4[c + 2] = pa_exp2(sc[e][nt][c + 2] - base);
+                                const float f = factor(e, nt, c);
+                                p4[c] = pa_exp2(fmaf(sc[e][nt][c], f, -m[nt][c]));
+                                p4[c + 2] = pa_exp2(fmaf(sc[e][nt][c + 2], f, -m[nt][c]));
                                 l[nt][c] += p4[c] + p4[c + 2];
                             }
-                            pb[e][nt][0] = pd_transpose(pg_pack2(p4[0] * vr, p4[1] * vr, (const __half *)nullptr));
-                            pb[e][nt][1] = pd_transpose(pg_pack2(p4[2] * vr, p4[3] * vr, (const __half *)nullptr));
+                            // (a product of halves: exact for scales that are powers of two)
+                            auto pack = [&](float x, float y) {
+                                const __half2 z = __hmul2(__floats2half2_rn(x, y), vr);
+                                return pd_transpose(*reinterpret_cast<const uint32_t *>(&z));
+                            };
+                            pb[e][nt][0] = pack(p4[0], p4[1]);
+                            pb[e][nt][1] = pack(p4[2], p4[3]);
                         }
                     }
 #pragma unroll
@@ -451,7 +469,7 @@ struct PdKernel {
                 __syncwarp();
                 issue();
             }
-            // ---- the eight warps' results of this piece
+            // ---- the warps' results of this piece
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -460,71 +478,68 @@ struct PdKernel {
                     for (int x = 4; x < 32; x <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], x);
                     if (g == 0) sm.m[warp][nt * 8 + 2 * t + c] = m[nt][c], sm.l[warp][nt * 8 + 2 * t + c] = l[nt][c];
                 }
-            const int end = u - s.off + s.nb;  // the unit after the item
-            const int c0 = (u - s.off) / share, c1 = (end - 1) / share;
+            const int c0 = s.first / share, c1 = (s.first + s.nb - 1) / share;  // the parts that hold steps of it
             float *slot = p.partials + ((size_t)blockIdx.x * 2 + ((int)blockIdx.x == c0 ? 1 : 0)) * (32 * (kPgDim + 2));
             __syncthreads();
+            // every warp's sums to the common maximum; the upper half of the warps' into the lower's
+            auto sums = [&](int nt, int c, int j) {
+                return reinterpret_cast<float4 *>(&sm.o[warp % (kPdWarps / 2)][nt * 8 + 2 * t + c][16 * g + 2 * j]);
+            };
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                // every warp's sums to the common maximum; the upper four warps' into the lower's
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const int r = nt * 8 + 2 * t + c;
-                    float top = -INFINITY;
+                    float top = kPdNone;
 #pragma unroll
                     for (int w = 0; w < kPdWarps; ++w) top = fmaxf(top, sm.m[w][r]);
-                    const float f = (top == -INFINITY ? 1.0f : pa_exp2(m[nt][c] - top)) * vref;
+                    const float f = pa_exp2(m[nt][c] - top) * vref;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) o[nt][j][c] *= f, o[nt][j][c + 2] *= f;
-                }
-                auto sums = [&](int c, int j) {
-                    return reinterpret_cast<float4 *>(&sm.o[warp % (kPdWarps / 2)][2 * t + c][16 * g + 2 * j]);
-                };
-                if (warp >= kPdWarps / 2) {
-#pragma unroll
-                    for (int c = 0; c < 2; ++c)
+                    if (warp >= kPdWarps / 2) {
 #pragma unroll
                         for (int j = 0; j < 8; j += 2)
-                            *sums(c, j) = make_float4(o[nt][j][c], o[nt][j][c + 2], o[nt][j + 1][c], o[nt][j + 1][c + 2]);
+                            *sums(nt, c, j) = make_float4(o[nt][j][c], o[nt][j][c + 2], o[nt][j + 1][c], o[nt][j + 1][c + 2]);
+                    }
                 }
-                __syncthreads();
-                if (warp < kPdWarps / 2) {
+            __syncthreads();
+            if (warp < kPdWarps / 2) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int c = 0; c < 2; ++c)
 #pragma unroll
                         for (int j = 0; j < 8; j += 2) {
-                            const float4 x = *sums(c, j);
-                            *sums(c, j) = make_float4(o[nt][j][c] + x.x, o[nt][j][c + 2] + x.y, o[nt][j + 1][c] + x.z,
-                                                      o[nt][j + 1][c + 2] + x.w);
+                            const float4 x = *sums(nt, c, j);
+                            *sums(nt, c, j) = make_float4(o[nt][j][c] + x.x, o[nt][j][c + 2] + x.y, o[nt][j + 1][c] + x.z,
+                                                          o[nt][j + 1][c + 2] + x.w);
                         }
-                }
-                __syncthreads();
-                {
-                    const int r = nt * 8 + warp;  // eight warps, eight rows
-                    float top = -INFINITY, sum_l = 0.0f;
-#pragma unroll
-                    for (int w = 0; w < kPdWarps; ++w) top = fmaxf(top, sm.m[w][r]);
-                    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-                    for (int w = 0; w < kPdWarps; ++w) {
-                        sum_l += sm.l[w][r] * (top == -INFINITY ? 1.0f : pa_exp2(sm.m[w][r] - top));
-                    }
-#pragma unroll
-                    for (int w = 0; w < kPdWarps / 2; ++w) {
-                        const float4 x = *reinterpret_cast<const float4 *>(&sm.o[w][warp][4 * lane]);
-                        acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
-                    }
-                    if (r < rows) {
-                        if (c0 == c1) {
-                            write_row(p, s, r, lane, acc, top, sum_l);
-                        } else {
-                            reinterpret_cast<float4 *>(slot + r * kPgDim)[lane] = acc;
-                            if (lane == 0) slot[32 * kPgDim + r] = top, slot[32 * kPgDim + 32 + r] = sum_l;
-                        }
-                    }
-                }
-                __syncthreads();
             }
+            __syncthreads();
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const int r = nt * 8 + warp;  // eight warps, eight rows of each group
+                float top = kPdNone, sum_l = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kPdWarps; ++w) top = fmaxf(top, sm.m[w][r]);
+                float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int w = 0; w < kPdWarps; ++w) sum_l += sm.l[w][r] * pa_exp2(sm.m[w][r] - top);
+#pragma unroll
+                for (int w = 0; w < kPdWarps / 2; ++w) {
+                    const float4 x = *reinterpret_cast<const float4 *>(&sm.o[w][r][4 * lane]);
+                    acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
+                }
+                if (r < rows) {
+                    if (c0 == c1) {
+                        write_row(p, s, r, lane, acc, top, sum_l);
+                    } else {
+                        reinterpret_cast<float4 *>(slot + r * kPgDim)[lane] = acc;
+                        if (lane == 0) slot[32 * kPgDim + r] = top, slot[32 * kPgDim + 32 + r] = sum_l;
+                    }
+                }
+            }
+            __syncthreads();
             if (c0 != c1) {
                 uint32_t *counter = p.counters + c0;
                 if (tid == 0) {
@@ -534,28 +549,56 @@ struct PdKernel {
                 }
                 __syncthreads();
                 if (sm.last) {
-                    for (int r = warp; r < rows; r += kPdWarps) {
-                        float top = -INFINITY, sum_l = 0.0f;
-                        auto at = [&](int c) {
-                            return p.partials + ((size_t)c * 2 + (c == c0 ? 1 : 0)) * (32 * (kPgDim + 2));
-                        };
-                        for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, __ldcg(at(c) + 32 * kPgDim + r));
-                        top = warp_max_butterfly(top);
-                        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-                        for (int c = c0; c <= c1; ++c) {
-                            const float *a = at(c);
-                            const float f = top == -INFINITY ? 1.0f : pa_exp2(__ldcg(a + 32 * kPgDim + r) - top);
-                            const float4 x = __ldcg(reinterpret_cast<const float4 *>(a + r * kPgDim) + lane);
-                            sum_l += f * __ldcg(a + 32 * kPgDim + 32 + r);
-                            acc.x += f * x.x, acc.y += f * x.y, acc.z += f * x.z, acc.w += f * x.w;
-                        }
-                        write_row(p, s, r, lane, acc, top, sum_l);
+                    // this warp's rows together, so that their reads of L2 overlap
+                    constexpr int kMine = (kRows + kPdWarps - 1) / kPdWarps;
+                    auto at = [&](int c) {
+                        return p.partials + ((size_t)c * 2 + (c == c0 ? 1 : 0)) * (32 * (kPgDim + 2));
+                    };
+                    float top[kMine], sum_l[kMine];
+                    float4 acc[kMine];
+#pragma unroll
+                    for (int i = 0; i < kMine; ++i) {
+                        top[i] = kPdNone, sum_l[i] = 0.0f;
+                        acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     }
+                    for (int c = c0 + lane; c <= c1; c += 32)
+#pragma unroll
+                        for (int i = 0; i < kMine; ++i)
+                            if (warp + i * kPdWarps < rows)
+                                top[i] = fmaxf(top[i], __ldcg(at(c) + 32 * kPgDim + warp + i * kPdWarps));
+#pragma unroll
+                    for (int i = 0; i < kMine; ++i) top[i] = warp_max_butterfly(top[i]);
+                    for (int cb = c0; cb <= c1; cb += 32) {  // 32 parts' factors, one a lane; then their rows
+                        float f[kMine], lc[kMine];
+#pragma unroll
+                        for (int i = 0; i < kMine; ++i) {
+                            f[i] = 0.0f, lc[i] = 0.0f;
+                            if (cb + lane <= c1 && warp + i * kPdWarps < rows) {
+                                const float *a = at(cb + lane) + 32 * kPgDim + warp + i * kPdWarps;
+                                f[i] = pa_exp2(__ldcg(a) - top[i]);
+                                lc[i] = f[i] * __ldcg(a + 32);
+                            }
+                        }
+                        const int n = min(32, c1 - cb + 1);
+#pragma unroll 4
+                        for (int c = 0; c < n; ++c) {
+#pragma unroll
+                            for (int i = 0; i < kMine; ++i) {
+                                float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                                if (warp + i * kPdWarps < rows)
+                                    x = __ldcg(reinterpret_cast<const float4 *>(at(cb + c) + (warp + i * kPdWarps) * kPgDim) + lane);
+                                const float fc = __shfl_sync(0xffffffffu, f[i], c);
+                                sum_l[i] += __shfl_sync(0xffffffffu, lc[i], c);
+                                acc[i].x += fc * x.x, acc[i].y += fc * x.y, acc[i].z += fc * x.z, acc[i].w += fc * x.w;
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < kMine; ++i)
+                        if (warp + i * kPdWarps < rows) write_row(p, s, warp + i * kPdWarps, lane, acc[i], top[i], sum_l[i]);
                     if (tid == 0) *counter = 0u;
                 }
             }
-            u += s.n;
         }
         if (failed)  // copies that came late must not land in another block's memory
             for (int i = used < kPdStages ? 0 : used - kPdStages; i < issued; ++i)
@@ -568,15 +611,14 @@ __global__ void __launch_bounds__(kPdThreads, 1)
     paged_attend_decode_kernel(const __grid_constant__ PaParams p, const __grid_constant__ CUtensorMap kmap,
                                const __grid_constant__ CUtensorMap vmap) {
     extern __shared__ uint8_t raw[];
-    PdShared &sm = *reinterpret_cast<PdShared *>(raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u));
+    PdShared<NT> &sm = *reinterpret_cast<PdShared<NT> *>(raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u));
     PdKernel<NT, T>::run(p, &kmap, &vmap, sm);
 }
 
-constexpr size_t kPdSmem = sizeof(PdShared) + 1024;
-static_assert(kPdSmem <= 227 * 1024, "shared memory");
-
 template <int NT, typename T>
 int pd_launch(const PaParams &p, const CUtensorMap &k, const CUtensorMap &v, cudaStream_t s) {
+    constexpr size_t kPdSmem = sizeof(PdShared<NT>) + 1024;
+    static_assert(kPdSmem <= 227 * 1024, "shared memory");
     static std::once_flag once[64];
     static cudaError_t set_rc[64];
     int dev = 0;
