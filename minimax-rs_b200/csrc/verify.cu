@@ -1,178 +1,346 @@
 // Verification of drafted tokens against the target's probabilities (mmrs_verify_drafts).
 //
-// rows_kernel: one CTA per logits row reads it once and leaves its maximum, sum of exp(x - max)
-// and argmax (x = logits / T).  choose_kernel: one CTA per sequence walks its rows' judgements
-// (a draft stands when u q < p), then runs the exponential race argmax r / e over the vocabulary
-// for the row that gives the next token.
+// With c = log2(e) / T a row's probabilities are 2^(c (l - max)) / sum, and the next token is the argmax
+// of r / e over the vocabulary (r: p, or what p has over q; e exponential: the first arrival of a race
+// in which token i runs at rate r_i).  Both need every logit of a row once; nothing else is long, so
+// the kernels are bound by HBM, or by the latency of two dependent passes where there are few rows.
+//   verify_rows_kernel    (row, chunk): one read of the chunk leaves its maximum, its sum of
+//                         exponentials and, for greedy rows, its argmax; a sequence's last block to
+//                         finish joins its rows' chunks (a few hundred bytes) and judges the drafts;
+//   verify_choose_kernel  (chunk, sequence): the race over a chunk of the row that gives the next token;
+//                         the sequence's last block to finish joins the chunks' winners.  It starts
+//                         while the first kernel drains, with its noise on the way.
+// 8192 tokens a block (16 a thread, in registers): 5 rows of 200064 make 125 blocks, 320 rows 8000.
+// Measured on B200 (200064 tokens): see the table of the operators' cases.
 #include <cuda_runtime.h>
 #include <math.h>
 
 #include "../../include/minimax_sample.h"
 #include "paged.cuh"
+#include "tma.cuh"
 
 namespace mmrs {
 namespace {
 
 constexpr int kVfThreads = 512;
 constexpr int kVfWarps = kVfThreads / 32;
+constexpr int kVfGroups = 4;                               // groups of four tokens a thread holds
+constexpr int kVfBlock = kVfThreads * kVfGroups * 4;       // tokens a block reads at once
+constexpr int kVfChunks = 32;                              // chunks of a row, at most
+constexpr float kVfLog2e = 1.4426950408889634f;
 
-struct VfRow {
-    float top, sum;            // maximum of x and sum of exp(x - top); sum 0: no usable row
-    unsigned long long best;   // lm_key of the largest logit
+struct VfPart {
+    float top, sum;           // maximum of the logits and sum of 2^(c (l - top)); NaN: a logit was
+    unsigned long long best;  // lm_key of the largest logit (greedy rows)
+};
+struct VfSeq {
+    unsigned long long best[kVfChunks];  // lm_key of the chunks' winners, 0: none
+    uint32_t rows_done, count;           // blocks done of either kernel, zero between calls
+    int stood;                           // drafts that stand
+    float top, sum;                      // of the row that gives the next token
+    int greedy_next;                     // its argmax
 };
 
 struct VfParams {
     const void *logits;
-    int vocab, num_seqs, total_rows, max_q;
+    int vocab, num_seqs, total_rows, max_q, chunks, chunk;  // tokens of a chunk
     const int32_t *cu, *draft;
     const float *q, *u, *noise, *temperature;
     int32_t *tokens, *accepted;
     float *logprobs;
-    VfRow *rows;
+    VfPart *parts;  // [row][chunk]
+    VfSeq *seqs;
     uint32_t *status;
 };
 
+__device__ __forceinline__ float vf_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Four elements at i (a multiple of 4) of a row of n: one read where the row is aligned for it.
 template <typename T>
-__device__ __forceinline__ float vf_logit(const void *p, long i) {
-    return pg_to_float(static_cast<const T *>(p)[i]);
+__device__ __forceinline__ void vf_load4(const T *row, int i, int n, float fill, float (&x)[4]) {
+    if (i + 4 <= n && ((uintptr_t)row & (4 * sizeof(T) - 1)) == 0) {
+        pg_load4(row + i, x);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = i + k < n ? pg_to_float(row[i + k]) : fill;
+    }
+}
+// (m, s) of two parts of a sum of exponentials with maxima m; -inf with sum 0 is nothing.
+__device__ __forceinline__ void vf_join(float &m, float &s, float m2, float s2, float c) {
+    const float top = fmaxf(m, m2), base = top == -INFINITY ? 0.0f : top;
+    s = s * vf_exp2((m - base) * c) + s2 * vf_exp2((m2 - base) * c);
+    m = top;
+}
+__device__ __forceinline__ float vf_temperature(const VfParams &p, int s) { return p.temperature ? p.temperature[s] : 1.0f; }
+__device__ __forceinline__ int vf_index(unsigned long long key) { return (int)(0xFFFFFFFFu - (uint32_t)key); }
+
+// The whole row's maximum, sum and argmax (one warp; lanes hold chunks).
+__device__ __forceinline__ VfPart vf_row(const VfParams &p, int row, int lane, float c) {
+    VfPart r{-INFINITY, 0.0f, 0};
+    if (lane < p.chunks) {
+        const VfPart *part = p.parts + (long)row * kVfChunks + lane;
+        r.top = __ldcg(&part->top), r.sum = __ldcg(&part->sum), r.best = __ldcg(&part->best);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        vf_join(r.top, r.sum, __shfl_xor_sync(0xffffffffu, r.top, o), __shfl_xor_sync(0xffffffffu, r.sum, o), c);
+        r.best = max(r.best, __shfl_xor_sync(0xffffffffu, r.best, o));
+    }
+    return r;
+}
+
+// The sequence's drafts judged (whole block): one warp a row.
+template <typename T>
+__device__ __forceinline__ void vf_judge(const VfParams &p, int s, int row0, int rows, float t0) {
+    __shared__ VfPart s_row[MMRS_VERIFY_MAX_Q];
+    __shared__ bool s_stands[MMRS_VERIFY_MAX_Q];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const bool greedy = t0 == 0.0f;
+    const float c = greedy ? kVfLog2e : kVfLog2e / t0;
+    for (int r = warp; r < rows; r += kVfWarps) {
+        const int row = row0 + r, at = row - s;
+        float l = 0.0f, q = 1.0f, u = 0.0f;
+        int tok = -1;
+        if (r < rows - 1 && at >= 0) {
+            tok = p.draft[at], u = p.u[at];
+            if (tok >= 0 && tok < p.vocab) {
+                l = pg_to_float(static_cast<const T *>(p.logits)[(long)row * p.vocab + tok]);
+                if (p.q) q = p.q[(long)at * p.vocab + tok];
+            }
+        }
+        const VfPart part = vf_row(p, row, lane, c);
+        if (lane == 0) {
+            s_row[r] = part;
+            const float pr = vf_exp2((l - part.top) * c) / part.sum;
+            s_stands[r] = part.sum > 0.0f && tok >= 0 && tok < p.vocab &&
+                          (greedy ? vf_index(part.best) == tok : u * q < pr);
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int n = 0;
+        while (n < rows - 1 && s_stands[n]) ++n;
+        VfSeq *seq = p.seqs + s;
+        seq->stood = n, seq->top = s_row[n].top, seq->sum = s_row[n].sum;
+        seq->greedy_next = vf_index(s_row[n].best);
+        seq->rows_done = 0;
+    }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kVfThreads) verify_rows_kernel(const VfParams p) {
     __shared__ float s_m[kVfWarps], s_s[kVfWarps];
     __shared__ unsigned long long s_b[kVfWarps];
+    __shared__ int s_last;
+    launch_dependents();
     const int row = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (row == 0 && blockIdx.y == 0 && threadIdx.x == 0) *p.status = MMRS_OK;
+    if (row >= p.total_rows) return;
+    const T *l = static_cast<const T *>(p.logits) + (long)row * p.vocab;
+    const int c0 = blockIdx.y * p.chunk, c1 = min(c0 + p.chunk, p.vocab);
+    float x[kVfGroups][4];
+#pragma unroll
+    for (int j = 0; j < kVfGroups; ++j)  // on the way while the row's sequence is looked up
+        vf_load4(l, c0 + (j * kVfThreads + threadIdx.x) * 4, c1, -INFINITY, x[j]);
     int s = 0;
     for (int s0 = 0; s0 < p.num_seqs; s0 += 32)
         s += __popc(__ballot_sync(0xffffffffu, s0 + lane < p.num_seqs && p.cu[s0 + lane + 1] <= row));
-    float t = p.temperature && s < p.num_seqs ? p.temperature[s] : 1.0f;
-    if (t == 0.0f) t = 1.0f;
-    float m = -INFINITY, sum = 0.0f;
-    unsigned long long best = 0;
-    bool bad = false;
-    for (int i = threadIdx.x; i < p.vocab; i += kVfThreads) {
-        const float l = vf_logit<T>(p.logits, (long)row * p.vocab + i), x = l / t;
-        bad = bad || !(l < INFINITY);
-        const unsigned long long key = lm_key(l, i);
-        best = key > best ? key : best;
-        if (x > m) {
-            sum = sum * expf(m - x) + 1.0f;
-            m = x;
-        } else if (x != -INFINITY) {
-            sum += expf(x - m);
+    if (s >= p.num_seqs) return;  // a row past the last sequence's
+    const float t = vf_temperature(p, s);
+    const bool greedy = t == 0.0f;
+    const float c = greedy ? kVfLog2e : kVfLog2e / t;
+    float m = -INFINITY, sum = 0.0f, best = -INFINITY;
+    int at = -1;
+    for (int i0 = c0;;) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < kVfGroups; ++j)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) top = fmaxf(top, x[j][k]);
+        if (greedy) {
+#pragma unroll
+            for (int j = 0; j < kVfGroups; ++j)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (x[j][k] > best) best = x[j][k], at = i0 + (j * kVfThreads + (int)threadIdx.x) * 4 + k;
         }
+        const float base = top == -INFINITY ? 0.0f : top;
+        float part = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kVfGroups; ++j)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) part += vf_exp2((x[j][k] - base) * c);  // an infinity leaves NaN here
+        vf_join(m, sum, top, part, c);
+        i0 += kVfBlock;
+        if (i0 >= c1) break;
+#pragma unroll
+        for (int j = 0; j < kVfGroups; ++j) vf_load4(l, i0 + (j * kVfThreads + threadIdx.x) * 4, c1, -INFINITY, x[j]);
     }
+    unsigned long long key = at >= 0 ? lm_key(best, at) : 0;
+#pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, sum, o);
-        const float mm = fmaxf(m, m2);
-        sum = mm == -INFINITY ? 0.0f : sum * expf(m - mm) + s2 * expf(m2 - mm);
-        m = mm;
-        const unsigned long long b2 = __shfl_xor_sync(0xffffffffu, best, o);
-        best = b2 > best ? b2 : best;
+        vf_join(m, sum, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, sum, o), c);
+        if (greedy) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
     }
-    bad = __syncthreads_or(bad);
-    if (lane == 0) s_m[warp] = m, s_s[warp] = sum, s_b[warp] = best;
+    if (lane == 0) s_m[warp] = m, s_s[warp] = sum, s_b[warp] = key;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < kVfWarps; ++w) {
-            const float mm = fmaxf(m, s_m[w]);
-            sum = mm == -INFINITY ? 0.0f : sum * expf(m - mm) + s_s[w] * expf(s_m[w] - mm);
-            m = mm;
-            best = s_b[w] > best ? s_b[w] : best;
+    if (warp == 0) {
+        m = lane < kVfWarps ? s_m[lane] : -INFINITY, sum = lane < kVfWarps ? s_s[lane] : 0.0f;
+        key = lane < kVfWarps ? s_b[lane] : 0;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            vf_join(m, sum, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, sum, o), c);
+            key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
         }
-        p.rows[row].top = m;
-        p.rows[row].sum = bad ? 0.0f : sum;
-        p.rows[row].best = best;
+        if (lane == 0) {
+            p.parts[(long)row * kVfChunks + blockIdx.y] = VfPart{m, sum, key};
+            const int row0 = max(p.cu[s], 0), rows = min(min(p.cu[s + 1], p.total_rows) - row0, p.max_q);
+            __threadfence();
+            // (rows past max_q are not counted)
+            s_last = row < row0 + rows && atomicAdd(&p.seqs[s].rows_done, 1u) + 1 == (uint32_t)rows * p.chunks;
+            __threadfence();
+        }
     }
+    __syncthreads();
+    if (!s_last) return;
+    const int row0 = max(p.cu[s], 0);
+    vf_judge<T>(p, s, row0, min(min(p.cu[s + 1], p.total_rows) - row0, p.max_q), t);
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kVfThreads) verify_choose_kernel(const VfParams p) {
+__global__ void __launch_bounds__(kVfThreads, 2) verify_choose_kernel(const VfParams p) {
     __shared__ unsigned long long s_b[kVfWarps];
-    const int s = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __shared__ int s_last;
+    const int s = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int row0 = max(p.cu[s], 0), rows = min(min(p.cu[s + 1], p.total_rows) - row0, p.max_q);
-    const float t0 = p.temperature ? p.temperature[s] : 1.0f, t = t0 == 0.0f ? 1.0f : t0;
+    const float t0 = vf_temperature(p, s), t = t0 == 0.0f ? 1.0f : t0, c = kVfLog2e / t;
+    const bool greedy = t0 == 0.0f;
+    const int c0 = blockIdx.x * p.chunk, c1 = min(c0 + p.chunk, p.vocab);
+    const float *noise = p.noise + (long)s * p.vocab;
+    float e[kVfGroups][4];
+    if (!greedy && rows > 0)
+#pragma unroll
+        for (int j = 0; j < kVfGroups; ++j) vf_load4(noise, c0 + (j * kVfThreads + threadIdx.x) * 4, c1, 1.0f, e[j]);
+    grid_dependency_wait();
     int32_t *tokens = p.tokens + (long)s * p.max_q;
     float *logprobs = p.logprobs ? p.logprobs + (long)s * p.max_q : nullptr;
-    for (int i = threadIdx.x; i < p.max_q; i += kVfThreads) {
-        tokens[i] = -1;
-        if (logprobs) logprobs[i] = 0.0f;
-    }
-    if (rows <= 0) {
-        if (threadIdx.x == 0) p.accepted[s] = 0;
+    const T *logits = static_cast<const T *>(p.logits);
+    VfSeq *seq = p.seqs + s;
+    const int n = rows > 0 ? __ldcg(&seq->stood) : 0;
+    const float top = __ldcg(&seq->top), sum = __ldcg(&seq->sum);
+    const int row = row0 + n, at = row - s;
+    const bool usable = rows > 0 && sum > 0.0f, fell = n < rows - 1 && at >= 0;
+    const T *l = logits + (long)row * p.vocab;
+    const float *q = fell && p.q ? p.q + (long)at * p.vocab : nullptr;
+    const int gone = fell && !p.q ? p.draft[at] : -1;
+    // the race over tokens [i0, i1) of the row; `own`: against the draft's probabilities
+    auto race = [&](int i0, int i1, bool first, bool own) {
+        const float inv = 1.0f / sum;
+        float best = 0.0f;
+        int win = -1;
+        for (; i0 < i1; i0 += kVfBlock, first = false) {
+            float x[kVfGroups][4], y[kVfGroups][4];
+#pragma unroll
+            for (int j = 0; j < kVfGroups; ++j) {
+                const int i = i0 + (j * kVfThreads + threadIdx.x) * 4;
+                vf_load4(l, i, i1, -INFINITY, x[j]);
+                if (own && q) vf_load4(q, i, i1, 0.0f, y[j]);
+                if (!first) vf_load4(noise, i, i1, 1.0f, e[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < kVfGroups; ++j)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int i = i0 + (j * kVfThreads + (int)threadIdx.x) * 4 + k;
+                    float r = vf_exp2((x[j][k] - top) * c) * inv;
+                    if (own) r = q ? r - y[j][k] : i == gone ? 0.0f : r;
+                    const float v = __fdividef(r, e[j][k]);
+                    if (r > 0.0f && v > best) best = v, win = i;  // indices rise: the first of equals stays
+                }
+        }
+        unsigned long long key = win >= 0 ? lm_key(best, win) : 0;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
+        __syncthreads();
+        if (lane == 0) s_b[warp] = key;
+        __syncthreads();
+        for (int w = 0; w < kVfWarps; ++w) key = max(key, s_b[w]);
+        return key;
+    };
+    if (usable && !greedy) {
+        const unsigned long long key = race(c0, c1, true, true);
+        if (threadIdx.x == 0) {
+            __stcg(&seq->best[blockIdx.x], key);
+            __threadfence();
+            s_last = atomicAdd(&seq->count, 1u) + 1 == gridDim.x;
+            __threadfence();
+        }
+        __syncthreads();
+        if (!s_last) return;
+    } else if (blockIdx.x > 0) {
         return;
     }
-    __syncthreads();
-    int n = 0;
-    for (; n < rows - 1; ++n) {  // every thread judges alike
-        const int row = row0 + n, at = row - s;
-        if (at < 0) break;
-        const int tok = p.draft[at];
-        const VfRow r = p.rows[row];
-        if (!(r.sum > 0.0f) || tok < 0 || tok >= p.vocab) break;
-        const float x = vf_logit<T>(p.logits, (long)row * p.vocab + tok) / t;
-        bool stands;
-        if (t0 == 0.0f) {
-            stands = tok == (int)(0xFFFFFFFFu - (uint32_t)r.best);
-        } else {
-            const float pr = expf(x - r.top) / r.sum, q = p.q ? p.q[(long)at * p.vocab + tok] : 1.0f;
-            stands = p.u[at] * q < pr;
-        }
-        if (!stands) break;
-        if (threadIdx.x == 0) {
-            tokens[n] = tok;
-            if (logprobs) logprobs[n] = (x - r.top) - logf(r.sum);
-        }
-    }
-    const int row = row0 + n;
-    const VfRow r = p.rows[row];
+    // one block a sequence from here on
     int next = -1;
-    if (r.sum > 0.0f && t0 == 0.0f) next = (int)(0xFFFFFFFFu - (uint32_t)r.best);
-    if (r.sum > 0.0f && t0 != 0.0f) {
-        const bool fell = n < rows - 1;
-        unsigned long long best = 0, plain = 0;
-        const int tok = fell && row >= s ? p.draft[row - s] : -1;
-        const float *q = fell && p.q && row >= s ? p.q + (long)(row - s) * p.vocab : nullptr;
-        for (int i = threadIdx.x; i < p.vocab; i += kVfThreads) {
-            const float x = vf_logit<T>(p.logits, (long)row * p.vocab + i) / t;
-            const float pr = expf(x - r.top) / r.sum;
-            float rest = q ? fmaxf(pr - q[i], 0.0f) : fell && !p.q && i == tok ? 0.0f : pr;
-            const float e = p.noise[(long)s * p.vocab + i];
-            if (rest > 0.0f) best = max(best, lm_key(rest / e, i));
-            if (pr > 0.0f) plain = max(plain, lm_key(pr / e, i));
-        }
-        for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-        for (int o = 16; o > 0; o >>= 1) plain = max(plain, __shfl_xor_sync(0xffffffffu, plain, o));
-        if (lane == 0) s_b[warp] = best;
-        __syncthreads();
-        for (int w = 0; w < kVfWarps; ++w) best = max(best, s_b[w]);
-        __syncthreads();
-        if (lane == 0) s_b[warp] = plain;
-        __syncthreads();
-        for (int w = 0; w < kVfWarps; ++w) plain = max(plain, s_b[w]);
-        if (!best) best = plain;
-        if (best) next = (int)(0xFFFFFFFFu - (uint32_t)best);
+    if (usable && greedy) next = __ldcg(&seq->greedy_next);
+    if (usable && !greedy) {
+        unsigned long long key = 0;
+        for (int i = 0; i < p.chunks; ++i) key = max(key, __ldcg(&seq->best[i]));
+        if (!key) key = race(0, p.vocab, false, false);  // nothing was left of p: the target's own race
+        if (key) next = vf_index(key);
+        if (threadIdx.x == 0) seq->count = 0;
     }
     if (threadIdx.x == 0) {
-        p.accepted[s] = n;
-        tokens[n] = next;
-        if (next < 0) atomicExch(p.status, (uint32_t)MMRS_ERR_NONFINITE);
-        if (next >= 0 && logprobs)
-            logprobs[n] = (vf_logit<T>(p.logits, (long)row * p.vocab + next) / t - r.top) - logf(r.sum);
+        p.accepted[s] = max(n, 0);
+        if (rows > 0 && next < 0) atomicExch(p.status, (uint32_t)MMRS_ERR_NONFINITE);
+    }
+    for (int i = warp; i < p.max_q; i += kVfWarps) {
+        const int tok = rows <= 0 || i > n ? -1 : i < n ? p.draft[row0 + i - s] : next;
+        float lp = 0.0f;
+        if (logprobs && tok >= 0) {
+            const VfPart part = vf_row(p, row0 + i, lane, c);
+            lp = (pg_to_float(logits[(long)(row0 + i) * p.vocab + tok]) - part.top) / t - logf(part.sum);
+        }
+        if (lane == 0) {
+            tokens[i] = tok;
+            if (logprobs) logprobs[i] = lp;
+        }
     }
 }
 
+struct VfLayout {
+    size_t seqs, parts, total;
+};
+VfLayout vf_layout(int num_seqs, int total_rows) {
+    VfLayout l;
+    l.seqs = 256;
+    l.parts = l.seqs + (sizeof(VfSeq) * num_seqs + 255) / 256 * 256;
+    l.total = l.parts + sizeof(VfPart) * kVfChunks * (size_t)total_rows;
+    return l;
+}
 size_t vf_workspace_bytes(int num_seqs, int total_rows) {
     if (num_seqs < 0 || num_seqs > MMRS_VERIFY_MAX_SEQS || total_rows < 0 || total_rows > MMRS_VERIFY_MAX_ROWS) return 0;
-    return 256 + sizeof(VfRow) * (size_t)total_rows;
+    return vf_layout(num_seqs, total_rows).total;
 }
 
 template <typename T>
 int vf_launch(const VfParams &p, cudaStream_t s) {
-    if (cudaMemsetAsync(p.status, 0, sizeof(uint32_t), s) != cudaSuccess) return MMRS_ERR_LAUNCH;
-    if (p.total_rows) verify_rows_kernel<T><<<p.total_rows, kVfThreads, 0, s>>>(p);
-    verify_choose_kernel<T><<<p.num_seqs, kVfThreads, 0, s>>>(p);
-    return cudaGetLastError() == cudaSuccess ? MMRS_OK : MMRS_ERR_LAUNCH;
+    // (at least one block of the first kernel: it resets the status)
+    verify_rows_kernel<T><<<dim3(p.total_rows > 0 ? p.total_rows : 1, p.chunks), kVfThreads, 0, s>>>(p);
+    if (cudaGetLastError() != cudaSuccess) return MMRS_ERR_LAUNCH;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.chunks, p.num_seqs);
+    cfg.blockDim = dim3(kVfThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, verify_choose_kernel<T>, p) == cudaSuccess ? MMRS_OK : MMRS_ERR_LAUNCH;
 }
 
 }  // namespace
@@ -213,8 +381,13 @@ extern "C" int mmrs_verify_drafts(const void *logits, int logits_type, int vocab
     p.cu = cu_rows, p.draft = draft_tokens;
     p.q = draft_probs, p.u = uniforms, p.noise = noise, p.temperature = temperature;
     p.tokens = tokens, p.accepted = accepted, p.logprobs = logprobs;
-    p.status = static_cast<uint32_t *>(workspace);
-    p.rows = reinterpret_cast<VfRow *>(static_cast<uint8_t *>(workspace) + 256);
+    p.chunk = vocab <= kVfChunks * kVfBlock ? kVfBlock : (vocab + kVfChunks * 4 - 1) / (kVfChunks * 4) * 4;
+    p.chunks = (vocab + p.chunk - 1) / p.chunk;
+    uint8_t *ws = static_cast<uint8_t *>(workspace);
+    const VfLayout l = vf_layout(num_seqs, total_rows);
+    p.status = reinterpret_cast<uint32_t *>(ws);
+    p.seqs = reinterpret_cast<VfSeq *>(ws + l.seqs);
+    p.parts = reinterpret_cast<VfPart *>(ws + l.parts);
     cudaStream_t s = (cudaStream_t)stream;
     if (logits_type == MMRS_TYPE_F32) return vf_launch<float>(p, s);
     return logits_type == MMRS_TYPE_F16 ? vf_launch<__half>(p, s) : vf_launch<__nv_bfloat16>(p, s);
