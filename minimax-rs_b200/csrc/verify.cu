@@ -43,7 +43,9 @@ struct VfSeq {
 
 struct VfParams {
     const void *logits;
-    int vocab, num_seqs, total_rows, max_q, chunks, chunk;  // tokens of a chunk
+    int vocab, num_seqs, total_rows, max_q;
+    int chunks, chunk;            // rows kernel: chunks of a row, tokens of a chunk
+    int race_chunks, race_chunk;  // choose kernel
     const int32_t *cu, *draft;
     const float *q, *u, *noise, *temperature;
     int32_t *tokens, *accepted;
@@ -68,6 +70,12 @@ __device__ __forceinline__ void vf_load4(const T *row, int i, int n, float fill,
         for (int k = 0; k < 4; ++k) x[k] = i + k < n ? pg_to_float(row[i + k]) : fill;
     }
 }
+// (m, s) of the warp's parts: one rescaling each, then plain sums.
+__device__ __forceinline__ void vf_join_warp(float &m, float &s, float c) {
+    const float top = warp_max_butterfly(m);
+    s = warp_sum_butterfly(s * vf_exp2((m - (top == -INFINITY ? 0.0f : top)) * c));
+    m = top;
+}
 // (m, s) of two parts of a sum of exponentials with maxima m; -inf with sum 0 is nothing.
 __device__ __forceinline__ void vf_join(float &m, float &s, float m2, float s2, float c) {
     const float top = fmaxf(m, m2), base = top == -INFINITY ? 0.0f : top;
@@ -84,11 +92,9 @@ __device__ __forceinline__ VfPart vf_row(const VfParams &p, int row, int lane, f
         const VfPart *part = p.parts + (long)row * kVfChunks + lane;
         r.top = __ldcg(&part->top), r.sum = __ldcg(&part->sum), r.best = __ldcg(&part->best);
     }
+    vf_join_warp(r.top, r.sum, c);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        vf_join(r.top, r.sum, __shfl_xor_sync(0xffffffffu, r.top, o), __shfl_xor_sync(0xffffffffu, r.sum, o), c);
-        r.best = max(r.best, __shfl_xor_sync(0xffffffffu, r.best, o));
-    }
+    for (int o = 16; o > 0; o >>= 1) r.best = max(r.best, __shfl_xor_sync(0xffffffffu, r.best, o));
     return r;
 }
 
@@ -131,7 +137,7 @@ __device__ __forceinline__ void vf_judge(const VfParams &p, int s, int row0, int
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kVfThreads) verify_rows_kernel(const VfParams p) {
+__global__ void __launch_bounds__(kVfThreads, 4) verify_rows_kernel(const VfParams p) {
     __shared__ float s_m[kVfWarps], s_s[kVfWarps];
     __shared__ unsigned long long s_b[kVfWarps];
     __shared__ int s_last;
@@ -180,21 +186,18 @@ __global__ void __launch_bounds__(kVfThreads) verify_rows_kernel(const VfParams 
         for (int j = 0; j < kVfGroups; ++j) vf_load4(l, i0 + (j * kVfThreads + threadIdx.x) * 4, c1, -INFINITY, x[j]);
     }
     unsigned long long key = at >= 0 ? lm_key(best, at) : 0;
+    vf_join_warp(m, sum, c);
+    if (greedy)
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        vf_join(m, sum, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, sum, o), c);
-        if (greedy) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
-    }
+        for (int o = 16; o > 0; o >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
     if (lane == 0) s_m[warp] = m, s_s[warp] = sum, s_b[warp] = key;
     __syncthreads();
     if (warp == 0) {
         m = lane < kVfWarps ? s_m[lane] : -INFINITY, sum = lane < kVfWarps ? s_s[lane] : 0.0f;
         key = lane < kVfWarps ? s_b[lane] : 0;
+        vf_join_warp(m, sum, c);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            vf_join(m, sum, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, sum, o), c);
-            key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
-        }
+        for (int o = 16; o > 0; o >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
         if (lane == 0) {
             p.parts[(long)row * kVfChunks + blockIdx.y] = VfPart{m, sum, key};
             const int row0 = max(p.cu[s], 0), rows = min(min(p.cu[s + 1], p.total_rows) - row0, p.max_q);
@@ -218,7 +221,7 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_choose_kernel(const VfPa
     const int row0 = max(p.cu[s], 0), rows = min(min(p.cu[s + 1], p.total_rows) - row0, p.max_q);
     const float t0 = vf_temperature(p, s), t = t0 == 0.0f ? 1.0f : t0, c = kVfLog2e / t;
     const bool greedy = t0 == 0.0f;
-    const int c0 = blockIdx.x * p.chunk, c1 = min(c0 + p.chunk, p.vocab);
+    const int c0 = blockIdx.x * p.race_chunk, c1 = min(c0 + p.race_chunk, p.vocab);
     const float *noise = p.noise + (long)s * p.vocab;
     float e[kVfGroups][4];
     if (!greedy && rows > 0)
@@ -288,7 +291,7 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_choose_kernel(const VfPa
     if (usable && greedy) next = __ldcg(&seq->greedy_next);
     if (usable && !greedy) {
         unsigned long long key = 0;
-        for (int i = 0; i < p.chunks; ++i) key = max(key, __ldcg(&seq->best[i]));
+        for (int i = 0; i < p.race_chunks; ++i) key = max(key, __ldcg(&seq->best[i]));
         if (!key) key = race(0, p.vocab, false, false);  // nothing was left of p: the target's own race
         if (key) next = vf_index(key);
         if (threadIdx.x == 0) seq->count = 0;
@@ -332,7 +335,7 @@ int vf_launch(const VfParams &p, cudaStream_t s) {
     verify_rows_kernel<T><<<dim3(p.total_rows > 0 ? p.total_rows : 1, p.chunks), kVfThreads, 0, s>>>(p);
     if (cudaGetLastError() != cudaSuccess) return MMRS_ERR_LAUNCH;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(p.chunks, p.num_seqs);
+    cfg.gridDim = dim3(p.race_chunks, p.num_seqs);
     cfg.blockDim = dim3(kVfThreads);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
@@ -381,8 +384,23 @@ extern "C" int mmrs_verify_drafts(const void *logits, int logits_type, int vocab
     p.cu = cu_rows, p.draft = draft_tokens;
     p.q = draft_probs, p.u = uniforms, p.noise = noise, p.temperature = temperature;
     p.tokens = tokens, p.accepted = accepted, p.logprobs = logprobs;
-    p.chunk = vocab <= kVfChunks * kVfBlock ? kVfBlock : (vocab + kVfChunks * 4 - 1) / (kVfChunks * 4) * 4;
+    // chunks of a row: of all numbers of them the one whose rounds of resident blocks (a block's beginning
+    // and end count as two reads of 8192 tokens) are the shortest in all, fewer chunks first
+    auto chunk_of = [&](long rows, int resident) {
+        const int most = (vocab + kVfBlock - 1) / kVfBlock;
+        long best = -1;
+        int chunk = 0;
+        for (int n = 1; n <= kVfChunks && n <= most; ++n) {
+            const int reads = (most + n - 1) / n;
+            const long rounds = (rows * ((most + reads - 1) / reads) + 148L * resident - 1) / (148L * resident);
+            const long cost = rounds * (reads + 2);
+            if (best < 0 || cost < best) best = cost, chunk = reads * kVfBlock;
+        }
+        return chunk;
+    };
+    p.chunk = chunk_of(total_rows, 4), p.race_chunk = chunk_of(num_seqs, 2);
     p.chunks = (vocab + p.chunk - 1) / p.chunk;
+    p.race_chunks = (vocab + p.race_chunk - 1) / p.race_chunk;
     uint8_t *ws = static_cast<uint8_t *>(workspace);
     const VfLayout l = vf_layout(num_seqs, total_rows);
     p.status = reinterpret_cast<uint32_t *>(ws);
