@@ -427,11 +427,17 @@ HEAD_DIM = 128  # MMRS_PAGED_HEAD_DIM
 PAGE_SIZES = (16, 32, 64, 128)
 
 
+_TYPE_CODES = {}  # torch dtype -> MMRS_TYPE_* (filled on first use: torch is imported lazily here)
+
+
 def _type_code(dtype) -> int:
-    import torch
-    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}.get(dtype)
+    code = _TYPE_CODES.get(dtype)
     if code is None:
-        raise MoeError(MMRS_ERR_UNSUPPORTED, f"element type {dtype}")
+        import torch
+        _TYPE_CODES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+        code = _TYPE_CODES.get(dtype)
+        if code is None:
+            raise MoeError(MMRS_ERR_UNSUPPORTED, f"element type {dtype}")
     return code
 
 
@@ -440,13 +446,23 @@ def _need(ok: bool, what: str) -> None:
         raise MoeError(MMRS_ERR_ARG, what)
 
 
+def _raw_stream(stream, t) -> int:
+    """The handle of `stream`, or of the current stream of t's device (without making a Stream object)."""
+    if stream is not None:
+        return stream.cuda_stream
+    import torch
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
 def _token_stride(t, heads: int, what: str) -> int:
     """Elements between the token rows of t [tokens][heads][128], whose rows are contiguous."""
-    if t.shape[0] == 0:
+    shape, stride = t.shape, t.stride()
+    n = shape[0]
+    if n == 0:
         return heads * HEAD_DIM
-    _need(t.dim() == 3 and t.shape[1] == heads and t.shape[2] == HEAD_DIM and t.stride(2) == 1 and
-          (heads == 1 or t.stride(1) == HEAD_DIM), f"{what}: [tokens][{heads}][{HEAD_DIM}], heads side by side")
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), heads * HEAD_DIM)
+    if len(shape) != 3 or shape[1] != heads or shape[2] != HEAD_DIM or stride[2] != 1 or (heads > 1 and stride[1] != HEAD_DIM):
+        raise MoeError(MMRS_ERR_ARG, f"{what}: [tokens][{heads}][{HEAD_DIM}], heads side by side")
+    return stride[0] if n > 1 else max(stride[0], heads * HEAD_DIM)
 
 
 class PagedBatch:
@@ -467,15 +483,18 @@ class PagedBatch:
         # a row stride larger than the row is only ever indexed up to max_len
         self.c = MmrsPagedBatch(cu_q.data_ptr(), seq_len.data_ptr(), page_table.data_ptr(), n,
                                 page_table.stride(0) if n > 1 else page_table.shape[1], total_q or 0, max_q, max_len)
+        self._ref = C.byref(self.c)
         self._pages = page_table.shape[1]
         self.max_len = max_len
 
     def bind(self, cache: "PagedKvCache", tokens: int):
         """The C struct for a call with `tokens` token rows."""
-        _need(self._pages * cache.page_size >= self.max_len or self.num_seqs == 0, "page_table: too few pages for max_len")
-        _need(self.total_q is None or self.total_q == tokens, "total_q")
+        if self._pages * cache.page_size < self.max_len and self.num_seqs:
+            raise MoeError(MMRS_ERR_ARG, "page_table: too few pages for max_len")
+        if self.total_q is not None and self.total_q != tokens:
+            raise MoeError(MMRS_ERR_ARG, "total_q")
         self.c.total_q = tokens
-        return C.byref(self.c)
+        return self._ref
 
 
 class PagedKvCache:
@@ -509,42 +528,54 @@ class PagedKvCache:
             raise MoeError(MMRS_ERR_UNSUPPORTED, f"page_size {self.page_size}")
         self.c = MmrsPagedCache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages,
                                 self.page_size, self.kv_heads)
-        self.ws = None
+        self._ref = C.byref(self.c)
+        self.ws, self._ws_need = None, {}  # workspace bytes by (sequences, tokens, query heads)
 
     def append(self, batch: PagedBatch, q, k, v, rope_cos, rope_sin, q_out=None, stream=None):
         """Writes the rotated k and v [tokens][kv_heads][128] (f32, f16 or bf16; row slices of one wider
         tensor will do) at the batch's positions; returns the rotated q (bf16 for bf16 queries, else
         f16; None for q None).  rope_cos / rope_sin: f32 [positions][rope_dim / 2]."""
-        import torch
-        n = k.shape[0]
-        _need(v.shape[0] == n and (q is None or q.shape[0] == n), "q, k, v: the same tokens")
-        code = _type_code(k.dtype)
-        _need(v.dtype == k.dtype and (q is None or q.dtype == k.dtype), "q, k, v: one element type")
-        _need(rope_cos.dtype == rope_sin.dtype == torch.float32 and rope_cos.shape == rope_sin.shape and
-              rope_cos.is_contiguous() and rope_sin.is_contiguous(), "rope_cos, rope_sin: f32 [positions][rope_dim / 2]")
+        n, dtype = k.shape[0], k.dtype
+        code = _type_code(dtype)
+        if v.shape[0] != n or v.dtype != dtype or (q is not None and (q.shape[0] != n or q.dtype != dtype)):
+            raise MoeError(MMRS_ERR_ARG, "q, k, v: the same tokens, one element type")
+        rope = rope_cos.shape
+        if (rope != rope_sin.shape or _type_code(rope_cos.dtype) or _type_code(rope_sin.dtype) or
+                not rope_cos.is_contiguous() or not rope_sin.is_contiguous()):
+            raise MoeError(MMRS_ERR_ARG, "rope_cos, rope_sin: f32 [positions][rope_dim / 2]")
         heads = q_stride = out_code = 0
+        q_ptr = out_ptr = None
         if q is not None:
             heads = q.shape[1]
             q_stride = _token_stride(q, heads, "q")
             if q_out is None:
+                import torch
                 q_out = torch.empty(n, heads, HEAD_DIM, device=q.device,
                                     dtype=torch.bfloat16 if code == 2 else torch.float16)
-            _need(q_out.shape == q.shape and q_out.is_contiguous(), "q_out: contiguous, shaped as q")
+            if q_out.shape != q.shape or not q_out.is_contiguous():
+                raise MoeError(MMRS_ERR_ARG, "q_out: contiguous, shaped as q")
             out_code = _type_code(q_out.dtype)
-        rc = lib().mmrs_paged_append(C.byref(self.c), batch.bind(self, n), _ptr(q), k.data_ptr(), v.data_ptr(), q_stride,
+            q_ptr, out_ptr = q.data_ptr(), q_out.data_ptr()
+        rc = lib().mmrs_paged_append(self._ref, batch.bind(self, n), q_ptr, k.data_ptr(), v.data_ptr(), q_stride,
                                      _token_stride(k, self.kv_heads, "k"), _token_stride(v, self.kv_heads, "v"), code,
-                                     heads, rope_cos.data_ptr(), rope_sin.data_ptr(), 2 * rope_cos.shape[1],
-                                     rope_cos.shape[0], _ptr(q_out), out_code, _stream(stream))
-        check(rc, "mmrs_paged_append")
+                                     heads, rope_cos.data_ptr(), rope_sin.data_ptr(), 2 * rope[1], rope[0], out_ptr,
+                                     out_code, _raw_stream(stream, k))
+        if rc:
+            raise MoeError(rc, "mmrs_paged_append")
         return q_out
 
     def workspace(self, num_seqs: int, tokens: int, query_heads: int):
-        import torch
-        need = lib().mmrs_paged_attend_workspace_bytes(num_seqs, tokens, query_heads, self.kv_heads)
-        if need == 0:
-            raise MoeError(MMRS_ERR_UNSUPPORTED, "mmrs_paged_attend_workspace_bytes")
+        key = (num_seqs, tokens, query_heads)
+        need = self._ws_need.get(key)
+        if need is None:
+            need = lib().mmrs_paged_attend_workspace_bytes(num_seqs, tokens, query_heads, self.kv_heads)
+            if need == 0:
+                raise MoeError(MMRS_ERR_UNSUPPORTED, "mmrs_paged_attend_workspace_bytes")
+            self._ws_need[key] = need
         if self.ws is None or self.ws.numel() < need:
+            import torch
             self.ws = torch.zeros(need, dtype=torch.uint8, device=self.k.device)
+            self._ws_ptr, self._ws_bytes = self.ws.data_ptr(), need
         return self.ws
 
     def status(self) -> int:
@@ -557,19 +588,24 @@ class PagedKvCache:
         each token's own; with window > 0 only the last `window` of them and the first `sinks`.  lse
         f32 [tokens][heads] is filled when given.  scale: 1 / sqrt(128) unless given.  The calls of
         one cache share a workspace: keep them on one stream."""
-        import torch
-        n, heads = q.shape[0], q.shape[1]
+        n, heads = q.shape[:2]
         stride = _token_stride(q, heads, "q")
         if out is None:
+            import torch
             out = torch.empty(n, heads, HEAD_DIM, dtype=q.dtype, device=q.device)
-        _need(out.shape == q.shape and out.dtype == q.dtype and out.is_contiguous(), "out: contiguous, shaped as q")
-        _need(lse is None or (lse.dtype == torch.float32 and lse.shape == q.shape[:2] and lse.is_contiguous()),
-              "lse: f32 [tokens][heads]")
-        ws = self.workspace(batch.num_seqs, n, heads)
-        rc = lib().mmrs_paged_attend(C.byref(self.c), batch.bind(self, n), q.data_ptr(), stride, _type_code(q.dtype),
-                                     heads, HEAD_DIM ** -0.5 if scale is None else scale, window, sinks, out.data_ptr(),
-                                     _ptr(lse), ws.data_ptr(), ws.numel(), _stream(stream))
-        check(rc, "mmrs_paged_attend")
+        elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+            raise MoeError(MMRS_ERR_ARG, "out: contiguous, shaped as q")
+        lse_ptr = None
+        if lse is not None:
+            if lse.shape != (n, heads) or _type_code(lse.dtype) or not lse.is_contiguous():
+                raise MoeError(MMRS_ERR_ARG, "lse: f32 [tokens][heads]")
+            lse_ptr = lse.data_ptr()
+        self.workspace(batch.num_seqs, n, heads)
+        rc = lib().mmrs_paged_attend(self._ref, batch.bind(self, n), q.data_ptr(), stride, _type_code(q.dtype), heads,
+                                     HEAD_DIM ** -0.5 if scale is None else scale, window, sinks, out.data_ptr(), lse_ptr,
+                                     self._ws_ptr, self._ws_bytes, _raw_stream(stream, q))
+        if rc:
+            raise MoeError(rc, "mmrs_paged_attend")
         return out
 
 
@@ -587,6 +623,7 @@ class DraftVerifier:
         self.tokens = torch.full((max_seqs, max_q), -1, dtype=torch.int32, device=device)
         self.accepted = torch.zeros(max_seqs, dtype=torch.int32, device=device)
         self.logprobs = torch.zeros(max_seqs, max_q, dtype=torch.float32, device=device)
+        self._ptrs = (self.tokens.data_ptr(), self.accepted.data_ptr(), self.logprobs.data_ptr(), self.ws.data_ptr(), need)
 
     def status(self) -> int:
         """MMRS_OK, or MMRS_ERR_NONFINITE when some next token of the last call is -1 (synchronous)."""
@@ -598,23 +635,33 @@ class DraftVerifier:
         (f32, f16, bf16), cu_rows int32 [n + 1], draft_tokens int32 and uniforms f32 [drafts],
         draft_probs f32 [drafts][vocab] or None (drafts that were certain), noise f32 [n][vocab]
         (exponential), temperature f32 [n] or None (1)."""
-        import torch
-        n, rows = cu_rows.numel() - 1, logits.shape[0]
-        _need(0 <= n <= self.max_seqs and rows <= self.max_rows, "more sequences or rows than the verifier was made for")
-        _need(logits.dim() == 2 and logits.shape[1] == self.vocab and logits.is_contiguous(), "logits [rows][vocab]")
-        _need(cu_rows.dtype == torch.int32 and draft_tokens.dtype == torch.int32, "cu_rows, draft_tokens: int32")
-        _need(uniforms.dtype == torch.float32 and uniforms.numel() == draft_tokens.numel() >= rows - n, "uniforms [drafts]")
-        _need(noise.dtype == torch.float32 and noise.shape == (n, self.vocab) and noise.is_contiguous(),
-              "noise f32 [n][vocab]")
-        _need(draft_probs is None or (draft_probs.dtype == torch.float32 and draft_probs.is_contiguous() and
-                                      draft_probs.shape == (draft_tokens.numel(), self.vocab)),
-              "draft_probs f32 [drafts][vocab]")
-        _need(temperature is None or (temperature.dtype == torch.float32 and temperature.numel() == n),
-              "temperature f32 [n]")
-        rc = lib().mmrs_verify_drafts(logits.data_ptr(), _type_code(logits.dtype), self.vocab, cu_rows.data_ptr(), n, rows,
-                                      self.max_q, draft_tokens.data_ptr(), _ptr(draft_probs), uniforms.data_ptr(),
-                                      noise.data_ptr(), _ptr(temperature), self.tokens.data_ptr(),
-                                      self.accepted.data_ptr(), self.logprobs.data_ptr(), self.ws.data_ptr(),
-                                      self.ws.numel(), _stream(stream))
-        check(rc, "mmrs_verify_drafts")
+        n, (rows, vocab) = cu_rows.numel() - 1, logits.shape
+        drafts = draft_tokens.numel()
+        if not 0 <= n <= self.max_seqs or rows > self.max_rows:
+            raise MoeError(MMRS_ERR_ARG, "more sequences or rows than the verifier was made for")
+        if vocab != self.vocab or not logits.is_contiguous():
+            raise MoeError(MMRS_ERR_ARG, "logits [rows][vocab]")
+        if cu_rows.dtype != self.tokens.dtype or draft_tokens.dtype != self.tokens.dtype:
+            raise MoeError(MMRS_ERR_ARG, "cu_rows, draft_tokens: int32")
+        f32 = self.logprobs.dtype
+        if uniforms.dtype != f32 or uniforms.numel() != drafts or drafts < rows - n:
+            raise MoeError(MMRS_ERR_ARG, "uniforms f32 [drafts]")
+        if noise.dtype != f32 or noise.shape != (n, vocab) or not noise.is_contiguous():
+            raise MoeError(MMRS_ERR_ARG, "noise f32 [n][vocab]")
+        probs_ptr = temp_ptr = None
+        if draft_probs is not None:
+            if draft_probs.dtype != f32 or draft_probs.shape != (drafts, vocab) or not draft_probs.is_contiguous():
+                raise MoeError(MMRS_ERR_ARG, "draft_probs f32 [drafts][vocab]")
+            probs_ptr = draft_probs.data_ptr()
+        if temperature is not None:
+            if temperature.dtype != f32 or temperature.numel() != n or not temperature.is_contiguous():
+                raise MoeError(MMRS_ERR_ARG, "temperature f32 [n]")
+            temp_ptr = temperature.data_ptr()
+        rc = lib().mmrs_verify_drafts(logits.data_ptr(), _type_code(logits.dtype), vocab, cu_rows.data_ptr(), n, rows,
+                                      self.max_q, draft_tokens.data_ptr(), probs_ptr, uniforms.data_ptr(),
+                                      noise.data_ptr(), temp_ptr, *self._ptrs, _raw_stream(stream, logits))
+        if rc:
+            raise MoeError(rc, "mmrs_verify_drafts")
+        if n == self.max_seqs:
+            return self.tokens, self.accepted, self.logprobs
         return self.tokens[:n], self.accepted[:n], self.logprobs[:n]
