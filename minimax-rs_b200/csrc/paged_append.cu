@@ -6,6 +6,13 @@
 // two with |x| <= 448 scale (448 = 1.75 * 2^8, the largest e4m3 value).  With powers of two a code
 // is x's own mantissa rounded to three bits, and a later, larger scale moves only the exponent:
 // rounding a page's older codes again changes nothing but e4m3 subnormals.
+//
+// Bound by HBM at prompt sizes and by a chain of dependent reads (lengths, page, scale, codes) for a
+// few tokens.  One launch: blocks of one (page run, KV head) first, then blocks of one token's
+// queries, whose reads are under way before the token's sequence and angle are looked up.  A run's
+// tokens are looked at twice (largest value, then codes): the first two of each warp stay in
+// registers, the others come from L2 again, which was faster than holding them all (128 registers,
+// 124-273 us) or none (129 us): 12390 tokens of f32, 48 + 8 heads, 587 MB in 107 us (5.5 TB/s).
 #include "paged.cuh"
 
 namespace mmrs {
@@ -13,6 +20,8 @@ namespace {
 
 constexpr int kApThreads = 128;
 constexpr int kApWarps = kApThreads / 32;
+constexpr int kApResident = 8;  // blocks an SM: 64 registers
+constexpr int kApHeld = 2;  // tokens that a warp keeps in registers between the two looks at them
 constexpr float kApMinScale = 5.421010862427522e-20f;  // 2^-64
 
 struct ApParams {
@@ -27,23 +36,49 @@ struct ApParams {
     int kv_units;  // page runs (an upper bound) times KV heads; the CTAs after them rotate queries
 };
 
-// Four columns of a head at `col`, rotated.
-template <typename T>
-__device__ __forceinline__ void ap_rotated4(const ApParams &p, const T *head, int col, int pos, float (&x)[4]) {
-    pg_load4(head + col, x);
+// A lane's four columns of every head of a token: the angles' cosines and sines, its own for the first
+// half of the rotated columns and signed for its partner's.
+struct ApAngle {
+    float c[4], s[4];  // rotated: x c + y s with y the partner column
+};
+__device__ __forceinline__ ApAngle ap_angle(const ApParams &p, int col, int pos) {
+    ApAngle a;
     const int half = p.rope_dim / 2;
-    if (col >= p.rope_dim) return;
     const long at = (long)pos * half;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int d = col + i;
-        if (d >= p.rope_dim) return;
-        const bool first = d < half;
-        const float c = p.cos[at + (first ? d : d - half)], s = p.sin[at + (first ? d : d - half)];
-        const float y = pg_to_float(head[first ? d + half : d - half]);
-        const float xc = __fmul_rn(x[i], c), ys = __fmul_rn(y, s);
-        x[i] = first ? __fsub_rn(xc, ys) : __fadd_rn(xc, ys);
+        a.c[i] = 1.0f, a.s[i] = 0.0f;
+        if (d < p.rope_dim) {
+            const bool first = d < half;
+            a.c[i] = p.cos[at + (first ? d : d - half)];
+            a.s[i] = p.sin[at + (first ? d : d - half)];
+            if (first) a.s[i] = -a.s[i];
+        }
     }
+    return a;
+}
+// Four columns of a head and their partners.
+template <typename T>
+__device__ __forceinline__ void ap_load4(const ApParams &p, const T *head, int col, float (&x)[4], float (&y)[4]) {
+    pg_load4(head + col, x);
+    if (col >= p.rope_dim) return;
+    const int half = p.rope_dim / 2;
+    if (half % 4 == 0) {  // the partners of four columns lie together
+        pg_load4(head + (col < half ? col + half : col - half), y);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int d = col + i;
+            y[i] = d < p.rope_dim ? pg_to_float(head[d < half ? d + half : d - half]) : 0.0f;
+        }
+    }
+}
+// Rotated: (a, b) -> (a c - b s, b c + a s), each product and sum rounded once.
+__device__ __forceinline__ void ap_rotate4(const ApParams &p, int col, const ApAngle &a, float (&x)[4], const float (&y)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (col + i < p.rope_dim) x[i] = __fadd_rn(__fmul_rn(x[i], a.c[i]), __fmul_rn(y[i], a.s[i]));
 }
 
 // Smallest power of two s with amax <= 448 s, at least 2^-64; 0 for 0.
@@ -110,18 +145,33 @@ __device__ void ap_store_run(const ApParams &p, int unit) {
     float kmax = 0.0f, vmax = 0.0f;
     auto load = [&](int pos, float (&kx)[4], float (&vx)[4]) {
         const long row = seq.row0 + pos - seq.pos0;
-        ap_rotated4(p, k + row * p.k_stride, col, min(pos, p.rope_positions - 1), kx);
+        float y[4];
         pg_load4(v + row * p.v_stride + col, vx);
+        ap_load4(p, k + row * p.k_stride, col, kx, y);
+        ap_rotate4(p, col, ap_angle(p, col, min(pos, p.rope_positions - 1)), kx, y);
         bool fine = true;
 #pragma unroll
         for (int i = 0; i < 4; ++i) fine = fine && isfinite(kx[i]) && isfinite(vx[i]);
         return __all_sync(0xffffffffu, fine) != 0;
     };
-    for (int pos = lo + warp; pos < hi; pos += kApWarps) {
-        float kx[4], vx[4];
-        if (!load(pos, kx, vx)) continue;
+    // the first look: the largest values (a warp's first kApHeld tokens stay in registers)
+    float kx[kApHeld][4], vx[kApHeld][4];
+    uint32_t fine = 0;
+    auto most = [&](const float (&x)[4], const float (&y)[4]) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) kmax = fmaxf(kmax, fabsf(kx[i])), vmax = fmaxf(vmax, fabsf(vx[i]));
+        for (int i = 0; i < 4; ++i) kmax = fmaxf(kmax, fabsf(x[i])), vmax = fmaxf(vmax, fabsf(y[i]));
+    };
+#pragma unroll
+    for (int t = 0; t < kApHeld; ++t) {
+        const int pos = lo + warp + t * kApWarps;
+        if (pos < hi && load(pos, kx[t], vx[t])) {
+            fine |= 1u << t;
+            most(kx[t], vx[t]);
+        }
+    }
+    for (int pos = lo + warp + kApHeld * kApWarps; pos < hi; pos += kApWarps) {
+        float x[4], y[4];
+        if (load(pos, x, y)) most(x, y);
     }
     kmax = warp_max_butterfly(kmax), vmax = warp_max_butterfly(vmax);
     if (lane == 0) s_max[0][warp] = kmax, s_max[1][warp] = vmax;
@@ -157,18 +207,37 @@ __device__ void ap_store_run(const ApParams &p, int unit) {
     }
     if (threadIdx.x == 0) *scales[0] = scale[0], *scales[1] = scale[1];
     const float kinv = ap_inverse(scale[0]), vinv = ap_inverse(scale[1]);
-    for (int pos = lo + warp; pos < hi; pos += kApWarps) {
-        float kx[4], vx[4];
-        const bool fine = load(pos, kx, vx);
+    auto store = [&](int pos, const float (&x)[4], const float (&y)[4], bool ok) {
         const long at4 = ((long)(pos - at * ps) * kPgDim + col) / 4;
-        reinterpret_cast<uint32_t *>(codes[0])[at4] = fine ? ap_codes4(kx, kinv) : 0x7f7f7f7fu;
-        reinterpret_cast<uint32_t *>(codes[1])[at4] = fine ? ap_codes4(vx, vinv) : 0u;
+        reinterpret_cast<uint32_t *>(codes[0])[at4] = ok ? ap_codes4(x, kinv) : 0x7f7f7f7fu;
+        reinterpret_cast<uint32_t *>(codes[1])[at4] = ok ? ap_codes4(y, vinv) : 0u;
+    };
+#pragma unroll
+    for (int t = 0; t < kApHeld; ++t) {
+        const int pos = lo + warp + t * kApWarps;
+        if (pos < hi) store(pos, kx[t], vx[t], (fine >> t) & 1);
+    }
+    for (int pos = lo + warp + kApHeld * kApWarps; pos < hi; pos += kApWarps) {
+        float x[4], y[4];
+        const bool ok = load(pos, x, y);
+        store(pos, x, y, ok);
     }
 }
 
 template <typename T, typename O>
 __device__ void ap_rotate_row(const ApParams &p, int row) {
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = lane * 4;
+    const T *q = static_cast<const T *>(p.q) + (long)row * p.q_stride;
+    O *out = static_cast<O *>(p.q_out) + (long)row * p.query_heads * kPgDim;
+    // a warp's first heads, under way while the row's sequence is looked up
+    constexpr int kAhead = 4;
+    float x[kAhead][4], y[kAhead][4];
+    auto load = [&](int h0) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i)
+            if (h0 + i * kApWarps < p.query_heads) ap_load4(p, q + (h0 + i * kApWarps) * kPgDim, col, x[i], y[i]);
+    };
+    load(warp);
     // the row's sequence: how many sequences end at or before it
     int s = 0;
     for (int s0 = 0; s0 < p.b.num_seqs; s0 += 32)
@@ -176,18 +245,24 @@ __device__ void ap_rotate_row(const ApParams &p, int row) {
     if (s >= p.b.num_seqs) return;
     const PgSeq seq = pg_seq(p.b, p.c.page_size, s);
     const int pos = min(max(seq.pos0 + row - seq.row0, 0), p.rope_positions - 1);
-    const T *q = static_cast<const T *>(p.q) + (long)row * p.q_stride;
-    O *out = static_cast<O *>(p.q_out) + (long)row * p.query_heads * kPgDim;
-    for (int i = threadIdx.x; i < p.query_heads * (kPgDim / 4); i += kApThreads) {
-        float x[4];
-        ap_rotated4(p, q + i / (kPgDim / 4) * kPgDim, i % (kPgDim / 4) * 4, pos, x);
-        const uint2 w = make_uint2(pg_pack2(x[0], x[1], out), pg_pack2(x[2], x[3], out));
-        reinterpret_cast<uint2 *>(out)[i] = w;
+    // a lane has the same columns of every head, so one angle serves them all
+    const ApAngle angle = ap_angle(p, col, pos);
+    for (int h0 = warp; h0 < p.query_heads;) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int h = h0 + i * kApWarps;
+            if (h >= p.query_heads) break;
+            ap_rotate4(p, col, angle, x[i], y[i]);
+            reinterpret_cast<uint2 *>(out + h * kPgDim)[lane] =
+                make_uint2(pg_pack2(x[i][0], x[i][1], out), pg_pack2(x[i][2], x[i][3], out));
+        }
+        h0 += kAhead * kApWarps;
+        load(h0);
     }
 }
 
 template <typename T, typename O>
-__global__ void __launch_bounds__(kApThreads) paged_append_kernel(const __grid_constant__ ApParams p) {
+__global__ void __launch_bounds__(kApThreads, kApResident) paged_append_kernel(const __grid_constant__ ApParams p) {
     if ((int)blockIdx.x < p.kv_units)
         ap_store_run<T>(p, blockIdx.x);
     else
