@@ -236,7 +236,6 @@ struct PdKernel {
             if ((lane >> 1) == (at & 15)) {  // the two lanes that know the step's groups
                 const uint32_t pair = 3u << (lane & ~1);
                 const int other = __shfl_xor_sync(pair, row, 1);
-                reinterpret_cast<float2 *>(&sm.meta[warp][st])[lane & 1] = make_float2(ks, vs);
                 uint64_t *bar = &sm.full[warp][st];
                 if (!(lane & 1)) {
                     const int n = (row >= 0) + (other >= 0);
@@ -250,6 +249,8 @@ struct PdKernel {
                     pa_tma_2d(sm.ring[warp][st][0] + half, kmap, 0, row, bar);
                     pa_tma_2d(sm.ring[warp][st][1] + half, vmap, 0, row, bar);
                 }
+                // (the scales' reads may still be under way: the copies do not wait for them)
+                reinterpret_cast<float2 *>(&sm.meta[warp][st])[lane & 1] = make_float2(ks, vs);
             }
             ++issued;
             in_i += kPdWarps;
@@ -561,26 +562,28 @@ struct PdKernel {
                         top[i] = kPdNone, sum_l[i] = 0.0f;
                         acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     }
-                    for (int c = c0 + lane; c <= c1; c += 32)
-#pragma unroll
-                        for (int i = 0; i < kMine; ++i)
-                            if (warp + i * kPdWarps < rows)
-                                top[i] = fmaxf(top[i], __ldcg(at(c) + 32 * kPgDim + warp + i * kPdWarps));
-#pragma unroll
-                    for (int i = 0; i < kMine; ++i) top[i] = warp_max_butterfly(top[i]);
                     for (int cb = c0; cb <= c1; cb += 32) {  // 32 parts' factors, one a lane; then their rows
                         float f[kMine], lc[kMine];
 #pragma unroll
                         for (int i = 0; i < kMine; ++i) {
-                            f[i] = 0.0f, lc[i] = 0.0f;
+                            f[i] = kPdNone, lc[i] = 0.0f;
                             if (cb + lane <= c1 && warp + i * kPdWarps < rows) {
                                 const float *a = at(cb + lane) + 32 * kPgDim + warp + i * kPdWarps;
-                                f[i] = pa_exp2(__ldcg(a) - top[i]);
-                                lc[i] = f[i] * __ldcg(a + 32);
+                                f[i] = __ldcg(a);
+                                lc[i] = __ldcg(a + 32);
                             }
                         }
+#pragma unroll
+                        for (int i = 0; i < kMine; ++i) {
+                            const float now = fmaxf(top[i], warp_max_butterfly(f[i])), less = pa_exp2(top[i] - now);
+                            top[i] = now;
+                            f[i] = pa_exp2(f[i] - now);
+                            lc[i] *= f[i];
+                            sum_l[i] *= less;
+                            acc[i].x *= less, acc[i].y *= less, acc[i].z *= less, acc[i].w *= less;
+                        }
                         const int n = min(32, c1 - cb + 1);
-#pragma unroll 4
+#pragma unroll kMine == 1 ? 8 : 4
                         for (int c = 0; c < n; ++c) {
 #pragma unroll
                             for (int i = 0; i < kMine; ++i) {
