@@ -1,6 +1,7 @@
 // Attention of new tokens over a paged e4m3 cache (mmrs_paged_attend): argument checks, workspace, and
-// the choice between the two kernels (paged_attend_decode.cu: up to 32 rows a KV head, bound by
-// HBM; paged_attend_prompt.cu: more, bound by arithmetic).
+// the choice between the two kernels (paged_attend_decode.cu: few rows a KV head, bound by HBM;
+// paged_attend_prompt.cu: many, bound by arithmetic; a call that may hold both runs both, each over its
+// sequences).
 #include <cuda_runtime.h>
 
 #include <mutex>
@@ -16,7 +17,7 @@ struct PaLayout {
     size_t counters, partials, total;
 };
 PaLayout pa_layout(int max_rows) {
-    const size_t sms = pa_sm_count(), rows = max_rows <= kPaDecodeRows ? kPaDecodeRows : 256;
+    const size_t sms = pa_sm_count(), rows = max_rows <= kPaFewRows ? kPaDecodeRows : 256;
     PaLayout l;
     l.counters = 256;
     l.partials = l.counters + (sizeof(uint32_t) * sms + 255) / 256 * 256;
@@ -101,18 +102,24 @@ extern "C" int mmrs_paged_attend(const MmrsPagedCache *cache, const MmrsPagedBat
     p.status = reinterpret_cast<uint32_t *>(ws);
     p.counters = reinterpret_cast<uint32_t *>(ws + l.counters);
     p.partials = reinterpret_cast<float *>(ws + l.partials);
-    // a sequence has no more rows than the call; work units are counted with 32 bits
+    // a sequence has no more rows than the call; the lengths themselves are on the device
     const long max_q = batch->max_q < batch->total_q ? batch->max_q : batch->total_q;
-    if (max_q * p.group <= kPaDecodeRows) {
-        if ((long)batch->num_seqs * cache->kv_heads * (batch->max_len / 16 + 32) > 0x3fffffffL) return MMRS_ERR_UNSUPPORTED;
-        p.b.max_q = (int)max_q;
-        CUtensorMap kmap, vmap;
-        const int rows = cache->page_size < 32 ? 16 : 32;
-        int mc = pa_make_map(&kmap, cache->k, *cache, rows);
-        if (mc == MMRS_OK) mc = pa_make_map(&vmap, cache->v, *cache, rows);
-        return mc != MMRS_OK ? mc : pa_launch_decode(p, kmap, vmap, type, (cudaStream_t)stream);
-    }
-    if (((long)batch->total_q * p.group / 256 + batch->num_seqs) * cache->kv_heads * (batch->max_len / 128 + 1) > 0x3fffffffL)
+    const long most = max_q * p.group, few = most < kPaFewRows ? most : kPaFewRows;
+    p.b.max_q = (int)max_q;
+    p.mixed = most > kPaFewRows;
+    p.few_rows = p.mixed && batch->num_seqs == 1 ? 0 : kPaFewRows;  // (one sequence: one kernel, whatever it brings)
+    // work units are counted with 32 bits
+    if ((long)batch->num_seqs * cache->kv_heads * (few / 8 + 1) * (batch->max_len / 32 + 32) > 0x3fffffffL ||
+        ((long)batch->total_q * p.group / 256 + batch->num_seqs) * cache->kv_heads * (batch->max_len / 128 + 1) > 0x3fffffffL)
         return MMRS_ERR_UNSUPPORTED;
-    return pa_launch_prompt(p, type, (cudaStream_t)stream);
+    if (p.mixed) {
+        const int rc2 = pa_launch_prompt(p, type, (cudaStream_t)stream);
+        if (rc2 != MMRS_OK || p.few_rows == 0) return rc2;
+    }
+    CUtensorMap kmap, vmap;
+    const int rows = cache->page_size < 32 ? 16 : 32;
+    int mc = pa_make_map(&kmap, cache->k, *cache, rows);
+    if (mc == MMRS_OK) mc = pa_make_map(&vmap, cache->v, *cache, rows);
+    if (mc != MMRS_OK) return mc;
+    return pa_launch_decode(p, kmap, vmap, type, (cudaStream_t)stream);
 }

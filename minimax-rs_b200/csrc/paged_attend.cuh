@@ -10,7 +10,11 @@
 namespace mmrs {
 
 constexpr int kPaMaxSeqs = MMRS_PAGED_MAX_SEQS;
-constexpr int kPaDecodeRows = 32;  // rows of a KV head up to which the decode kernel runs
+constexpr int kPaDecodeRows = 32;  // rows of an item of the decode kernel, at most
+// Rows of a KV head up to which a sequence is the decode kernel's: it takes 250 us for 30 rows of 64
+// sequences (300000 positions, 8 heads), with each further group of 32 as long again, the prompt kernel
+// 880 us for any number up to 128.
+constexpr int kPaFewRows = 96;
 constexpr float kPaLog2e = 1.4426950408889634f;
 constexpr float kPaLn2 = 0.6931471805599453f;
 constexpr uint64_t kPaTimeoutNs = 2000000000ull;
@@ -23,6 +27,8 @@ struct PaParams {
     float *lse;
     long q_stride;
     int query_heads, group, window, sinks;
+    int few_rows;  // sequences of at most this many rows a KV head are the decode kernel's, others the prompt kernel's
+    bool mixed;    // both kernels run
     float scale_log2;     // scale * log2(e)
     uint32_t *status;     // workspace: status word
     uint32_t *counters;   // workspace: one per CTA (for the item it begins and others end), zero between calls

@@ -1,4 +1,4 @@
-// Paged attention for few rows: single tokens and drafted tokens (at most 32 rows a KV head).
+// Paged attention for few rows: single tokens and drafted tokens (at most kPaFewRows rows a KV head).
 //
 // Each K / V code is read once and used for all rows of its KV head, so the kernel is bound by HBM:
 // 256 bytes a position and head.  The products run on mma.sync with the operands turned round, S^T =
@@ -68,10 +68,11 @@ __device__ __forceinline__ uint32_t pd_transpose(uint32_t x) {
 __device__ __forceinline__ uint4 pd_lds(const uint8_t *tile, int row, int chunk) {
     return *reinterpret_cast<const uint4 *>(tile + row * kPgDim + ((chunk ^ (row & 7)) << 4));
 }
-// An item's piece in this CTA's part of the list: sequence b, KV head h, steps [off, off + n) of the
-// item's nb; the item's first step is unit `first` of the list, after its cost.
+// An item's piece in this CTA's part of the list: sequence b, KV head h, rows [row0, row0 + kRows) of
+// the sequence's, steps [off, off + n) of the item's nb; the item's first step is unit `first` of the
+// list, after its cost.
 struct PdSeg {
-    int b, h, off, n, nb, first;
+    int b, h, row0, off, n, nb, first;
     PgSeq seq;
     PaSpan<kPdStep> span;
 };
@@ -84,8 +85,15 @@ struct PdKernel {
 
     static __device__ int item_steps(const PaParams &p, int b, PgSeq &seq, PaSpan<kPdStep> &span) {
         seq = pg_seq(p.b, p.c.page_size, b);
+        if (seq.count * p.group > p.few_rows) seq.count = 0;  // the other kernel's
         span = pa_span<kPdStep>(max(seq.pos0, 0), seq.len - 1, p.window, p.sinks);
         return seq.count > 0 ? max(span.n, 1) + kPdItemCost : 0;  // rows that see nothing are written too
+    }
+
+    // Groups of kRows rows: items of their own, next to each other in the list (the second finds the codes
+    // in L2).
+    static __device__ __forceinline__ int groups(const PaParams &p, const PgSeq &seq) {
+        return (seq.count * p.group + kRows - 1) / kRows;
     }
 
     // The piece that starts at unit u (< end, the CTA's end; `total` units in all).
@@ -99,14 +107,16 @@ struct PdKernel {
         s.b = lo;
         const int units = item_steps(p, lo, s.seq, s.span), at = u - sm.prefix[lo];
         s.nb = units - kPdItemCost;
-        s.h = at / units;
-        s.first = sm.prefix[lo] + s.h * units + kPdItemCost;
+        const int item = at / units, of_head = groups(p, s.seq);
+        s.h = item / of_head;
+        s.row0 = (item - s.h * of_head) * kRows;
+        s.first = sm.prefix[lo] + item * units + kPdItemCost;
         s.off = max(u - s.first, 0);
         s.n = min(s.nb, end - s.first) - s.off;  // not positive: only the item's cost lies before `end`
     }
 
     static __device__ void load_q(const PaParams &p, const PdSeg &s, int lane, int nt, uint32_t (&f)[16], float &factor) {
-        const int r = nt * 8 + (lane >> 2), t = lane & 3;
+        const int r = s.row0 + nt * 8 + (lane >> 2), t = lane & 3;
         factor = 1.0f;
         if (r >= s.seq.count * p.group) {
 #pragma unroll
@@ -144,6 +154,7 @@ struct PdKernel {
 
     static __device__ void write_row(const PaParams &p, const PdSeg &s, int r, int lane, float4 o, float m, float l) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        r += s.row0;
         const long at = (long)(s.seq.row0 + r / p.group) * p.query_heads + s.h * p.group + r % p.group;
         T *out = static_cast<T *>(p.out) + at * kPgDim;
         reinterpret_cast<uint2 *>(out)[lane] =
@@ -166,6 +177,7 @@ struct PdKernel {
             PgSeq seq;
             PaSpan<kPdStep> span;
             mine[i] = b < p.b.num_seqs ? item_steps(p, b, seq, span) * p.c.kv_heads : 0;
+            if (mine[i]) mine[i] *= groups(p, seq);
             sum += mine[i];
         }
         int incl = sum;
@@ -264,7 +276,7 @@ struct PdKernel {
             seek(p, sm, u, u1, s);
             u = s.first + s.nb;
             if (s.n <= 0) continue;
-            const int rows = min(s.seq.count * p.group, kRows);
+            const int rows = min(s.seq.count * p.group - s.row0, kRows);
             uint32_t qf[kQShared ? 1 : NT][16];
             float qs[NT][2];  // the score's factor for this lane's two columns
             int pos[NT][2];
@@ -305,7 +317,7 @@ struct PdKernel {
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const int r = nt * 8 + 2 * t + c;
-                    pos[nt][c] = r < rows ? s.seq.pos0 + r / p.group : -1;
+                    pos[nt][c] = r < rows ? s.seq.pos0 + (s.row0 + r) / p.group : -1;
                 }
             const int pos_lo = s.seq.pos0, pos_hi = s.seq.len - 1;
             float m[NT][2], l[NT][2], o[NT][8][4];  // per column; the maximum kPdNone before the first score
@@ -637,7 +649,10 @@ int pd_launch(const PaParams &p, const CUtensorMap &k, const CUtensorMap &v, cud
 
 template <typename T>
 int pd_launch_rows(const PaParams &p, const CUtensorMap &k, const CUtensorMap &v, cudaStream_t s) {
-    const int rows = p.b.max_q * p.group;
+    // the fewest items a sequence, of equal size; next to prompts in one call, where single tokens or drafts
+    // may be there, 16 rows
+    const int most = p.b.max_q * p.group, items = (most + kPaDecodeRows - 1) / kPaDecodeRows;
+    const int rows = p.mixed ? 16 : (most + items - 1) / items;
     if (rows <= 8) return pd_launch<1, T>(p, k, v, s);
     if (rows <= 16) return pd_launch<2, T>(p, k, v, s);
     if (rows <= 24) return pd_launch<3, T>(p, k, v, s);

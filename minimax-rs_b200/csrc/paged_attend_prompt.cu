@@ -242,9 +242,9 @@ __device__ __forceinline__ int pp_tiles(const PaParams &p, const PgSeq &seq, int
     span = pa_span<kPpKeys>(lo, max(hi, -1), p.window, p.sinks);
     return max(span.n, 1);  // rows that see nothing are written too
 }
-// Units of one KV head of a sequence (whole warp).
+// Units of one KV head of a sequence (whole warp); none of one that is the decode kernel's.
 __device__ int pp_seq_units(const PaParams &p, const PgSeq &seq, int lane) {
-    const int tiles = (seq.count * p.group + kPpRows - 1) / kPpRows;
+    const int tiles = seq.count * p.group <= p.few_rows ? 0 : (seq.count * p.group + kPpRows - 1) / kPpRows;
     int sum = 0;
     PaSpan<kPpKeys> span;
 #pragma unroll 1
