@@ -454,6 +454,22 @@ def _raw_stream(stream, t) -> int:
     return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
+def _on_stream(stream):
+    """Where a call allocates: on the stream it runs on, which then owns the memory."""
+    import contextlib
+    import torch
+    return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
+
+
+def _same_device(dev: int, *tensors) -> None:
+    """The kernels follow raw pointers: every tensor of a call lies on one GPU."""
+    if dev < 0:
+        raise MoeError(MMRS_ERR_ARG, "tensors on a GPU")
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise MoeError(MMRS_ERR_ARG, f"tensors on GPU {dev}")
+
+
 def _token_stride(t, heads: int, what: str) -> int:
     """Elements between the token rows of t [tokens][heads][128], whose rows are contiguous."""
     shape, stride = t.shape, t.stride()
@@ -478,6 +494,7 @@ class PagedBatch:
         _need(cu_q.numel() == n + 1 and cu_q.is_contiguous() and seq_len.is_contiguous(), "cu_q [n + 1], seq_len [n]")
         _need(page_table.dim() == 2 and page_table.shape[0] == n and (page_table.stride(1) == 1 or n == 0),
               "page_table [n][pages]")
+        _same_device(seq_len.get_device(), cu_q, page_table)
         self.t = (cu_q, seq_len, page_table)
         self.num_seqs, self.total_q = n, total_q
         # a row stride larger than the row is only ever indexed up to max_len
@@ -523,6 +540,9 @@ class PagedKvCache:
         _need(k_scale.shape == v_scale.shape == k.shape[:2] and k_scale.dtype == v_scale.dtype == torch.float32 and
               k_scale.is_contiguous() and v_scale.is_contiguous(), "k_scale, v_scale: f32 [pages][kv_heads]")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.device_index = k.get_device()  # -1: no GPU's, which append and attend refuse
+        if self.device_index >= 0:
+            _same_device(self.device_index, v, k_scale, v_scale)
         pages, self.kv_heads, self.page_size = k.shape[:3]
         if self.page_size not in PAGE_SIZES:
             raise MoeError(MMRS_ERR_UNSUPPORTED, f"page_size {self.page_size}")
@@ -537,6 +557,7 @@ class PagedKvCache:
         f16; None for q None).  rope_cos / rope_sin: f32 [positions][rope_dim / 2]."""
         n, dtype = k.shape[0], k.dtype
         code = _type_code(dtype)
+        _same_device(self.device_index, batch.t[1], q, k, v, rope_cos, rope_sin, q_out)
         if v.shape[0] != n or v.dtype != dtype or (q is not None and (q.shape[0] != n or q.dtype != dtype)):
             raise MoeError(MMRS_ERR_ARG, "q, k, v: the same tokens, one element type")
         rope = rope_cos.shape
@@ -550,8 +571,9 @@ class PagedKvCache:
             q_stride = _token_stride(q, heads, "q")
             if q_out is None:
                 import torch
-                q_out = torch.empty(n, heads, HEAD_DIM, device=q.device,
-                                    dtype=torch.bfloat16 if code == 2 else torch.float16)
+                with _on_stream(stream):
+                    q_out = torch.empty(n, heads, HEAD_DIM, device=q.device,
+                                        dtype=torch.bfloat16 if code == 2 else torch.float16)
             if q_out.shape != q.shape or not q_out.is_contiguous():
                 raise MoeError(MMRS_ERR_ARG, "q_out: contiguous, shaped as q")
             out_code = _type_code(q_out.dtype)
@@ -564,7 +586,8 @@ class PagedKvCache:
             raise MoeError(rc, "mmrs_paged_append")
         return q_out
 
-    def workspace(self, num_seqs: int, tokens: int, query_heads: int):
+    def workspace(self, num_seqs: int, tokens: int, query_heads: int, stream=None):
+        """The attention's workspace, large enough for such a call; a new one is zeroed on `stream`."""
         key = (num_seqs, tokens, query_heads)
         need = self._ws_need.get(key)
         if need is None:
@@ -574,7 +597,8 @@ class PagedKvCache:
             self._ws_need[key] = need
         if self.ws is None or self.ws.numel() < need:
             import torch
-            self.ws = torch.zeros(need, dtype=torch.uint8, device=self.k.device)
+            with _on_stream(stream):
+                self.ws = torch.zeros(need, dtype=torch.uint8, device=self.k.device)
             self._ws_ptr, self._ws_bytes = self.ws.data_ptr(), need
         return self.ws
 
@@ -590,9 +614,11 @@ class PagedKvCache:
         one cache share a workspace: keep them on one stream."""
         n, heads = q.shape[:2]
         stride = _token_stride(q, heads, "q")
+        _same_device(self.device_index, batch.t[1], q, out, lse)
         if out is None:
             import torch
-            out = torch.empty(n, heads, HEAD_DIM, dtype=q.dtype, device=q.device)
+            with _on_stream(stream):
+                out = torch.empty(n, heads, HEAD_DIM, dtype=q.dtype, device=q.device)
         elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
             raise MoeError(MMRS_ERR_ARG, "out: contiguous, shaped as q")
         lse_ptr = None
@@ -600,7 +626,7 @@ class PagedKvCache:
             if lse.shape != (n, heads) or _type_code(lse.dtype) or not lse.is_contiguous():
                 raise MoeError(MMRS_ERR_ARG, "lse: f32 [tokens][heads]")
             lse_ptr = lse.data_ptr()
-        self.workspace(batch.num_seqs, n, heads)
+        self.workspace(batch.num_seqs, n, heads, stream)
         rc = lib().mmrs_paged_attend(self._ref, batch.bind(self, n), q.data_ptr(), stride, _type_code(q.dtype), heads,
                                      HEAD_DIM ** -0.5 if scale is None else scale, window, sinks, out.data_ptr(), lse_ptr,
                                      self._ws_ptr, self._ws_bytes, _raw_stream(stream, q))
@@ -641,10 +667,12 @@ class DraftVerifier:
             raise MoeError(MMRS_ERR_ARG, "more sequences or rows than the verifier was made for")
         if vocab != self.vocab or not logits.is_contiguous():
             raise MoeError(MMRS_ERR_ARG, "logits [rows][vocab]")
-        if cu_rows.dtype != self.tokens.dtype or draft_tokens.dtype != self.tokens.dtype:
-            raise MoeError(MMRS_ERR_ARG, "cu_rows, draft_tokens: int32")
-        f32 = self.logprobs.dtype
-        if uniforms.dtype != f32 or uniforms.numel() != drafts or drafts < rows - n:
+        _same_device(self.tokens.get_device(), logits, cu_rows, draft_tokens, uniforms, noise, draft_probs, temperature)
+        i32, f32 = self.tokens.dtype, self.logprobs.dtype
+        if (cu_rows.dtype != i32 or draft_tokens.dtype != i32 or not cu_rows.is_contiguous() or
+                not draft_tokens.is_contiguous()):
+            raise MoeError(MMRS_ERR_ARG, "cu_rows, draft_tokens: contiguous int32")
+        if uniforms.dtype != f32 or uniforms.numel() != drafts or drafts < rows - n or not uniforms.is_contiguous():
             raise MoeError(MMRS_ERR_ARG, "uniforms f32 [drafts]")
         if noise.dtype != f32 or noise.shape != (n, vocab) or not noise.is_contiguous():
             raise MoeError(MMRS_ERR_ARG, "noise f32 [n][vocab]")

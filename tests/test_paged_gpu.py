@@ -51,6 +51,33 @@ def test_attend_drafts(pkg, dev, group, kv, seqs):
     check_attend(pkg, dev, c, group * kv, torch.bfloat16)
 
 
+@pytest.mark.parametrize("page", [16, 128])
+@pytest.mark.parametrize("group,new", [(6, 6), (6, 11), (6, 16), (16, 3), (16, 6), (1, 33), (1, 64), (1, 65), (1, 96),
+                                       (1, 97), (5, 19), (5, 20)])
+def test_attend_rows_around_the_kernels_bounds(pkg, dev, page, group, new):
+    """33 to 100 rows a KV head: groups of 32 of the one kernel up to 96, the other kernel from there."""
+    c = Case([(new, 400), (new, new), (1, 77), (new - 1, 1000)], page, 2, seed=page + new)
+    c.spoil_unused()
+    check_attend(pkg, dev, c, 2 * group, torch.float16)
+
+
+@pytest.mark.parametrize("page", [16, 32, 64])
+@pytest.mark.parametrize("group,kv", [(6, 2), (16, 1), (1, 2)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (100, 4)])
+def test_attend_tokens_drafts_and_prompts_together(pkg, dev, page, group, kv, window, sinks):
+    """One call that both kernels serve; an empty sequence between them."""
+    c = Case([(1, 500), (5, 310), (300, 450), (0, 20), (1, 1), (17, 17), (130, 130), (1, 900)], page, kv, seed=page + group)
+    c.spoil_unused()
+    check_attend(pkg, dev, c, group * kv, torch.bfloat16, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("new", [1, 5, 150])
+@pytest.mark.parametrize("scale", [-0.1, 0.0])
+def test_attend_negative_and_zero_scale(pkg, dev, new, scale):
+    c = Case([(new, 333), (new, 190)], 32, 2, seed=new)
+    check_attend(pkg, dev, c, 12, torch.float16, scale=scale)
+
+
 @pytest.mark.parametrize("page", [16, 64, 128])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("group,kv,seqs", [(6, 2, [(129, 129), (300, 900)]), (1, 2, [(257, 1000), (1, 513)]),
@@ -135,6 +162,25 @@ def test_attend_strided_queries_on_another_stream(pkg, dev, new):
     stream.synchronize()
     bound, _ = attend_bounds(c, ref, size, reach, torch.float16)
     assert ((out.cpu().double() - ref).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_first_call_on_another_stream(pkg, dev, new):
+    """Workspace and outputs are made on the stream of the call, not on the current one, which is busy here."""
+    c = Case([(new, 333), (new, 190)], 64, 2, seed=new)
+    q = c.randn(c.tokens, 12, D).to(torch.float16)
+    ref, _, size, reach = attend64(c, q)
+    q_dev, cache, batch = q.to(dev), c.cache(pkg, dev), c.batch(pkg, dev)
+    stream, big = torch.cuda.Stream(), torch.empty(1 << 28, device=dev)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        big.normal_()
+    out = cache.attend(batch, q_dev, stream=stream)
+    stream.synchronize()
+    with torch.cuda.stream(stream):
+        got = out.cpu().double()
+    bound, _ = attend_bounds(c, ref, size, reach, torch.float16)
+    assert ((got - ref).abs() <= bound).all() and cache.status() == pkg.MMRS_OK
 
 
 def test_attend_same_call_with_looser_bounds(pkg, dev):

@@ -126,3 +126,21 @@ def test_python_checks(pkg):
         pkg.PagedBatch(i32, i32[:2], torch.zeros(2, 1, dtype=torch.int32), max_q=1, max_len=1)
     with pytest.raises(pkg.MoeError):
         pkg.DraftVerifier(100, "cpu", max_seqs=0, max_rows=1, max_q=1)
+
+
+def test_python_calls_refuse_tensors_that_are_not_on_the_gpu(pkg):
+    """A raw pointer to host memory would fault the device: the wrappers ask before they call."""
+    import types
+
+    import torch
+    i32 = torch.zeros(3, dtype=torch.int32)
+    batch = types.SimpleNamespace(t=(i32, i32[:2], torch.zeros(2, 1, dtype=torch.int32)), num_seqs=2)
+    cache = pkg.PagedKvCache(2, "cpu", kv_heads=2, page_size=16)
+    q, k, rope = torch.zeros(2, 12, 128), torch.zeros(2, 2, 128), torch.zeros(16, 32)
+    with pytest.raises(pkg.MoeError, match="GPU"):
+        cache.append(batch, q, k, k, rope, rope)
+    with pytest.raises(pkg.MoeError, match="GPU"):
+        cache.attend(batch, q.half())
+    ver = pkg.DraftVerifier(100, "cpu", max_seqs=2, max_rows=4, max_q=2)
+    with pytest.raises(pkg.MoeError, match="GPU"):
+        ver.verify(torch.zeros(4, 100), i32, i32[:2], torch.zeros(2), torch.ones(2, 100))
