@@ -29,8 +29,9 @@ extern "C" {
 #define MMRS_TYPE_F16 1
 #define MMRS_TYPE_BF16 2
 
-/* The cache of one layer.  A key (value) is its e4m3 code times the scale of its page and head;
- * NaN codes mark a token that was not finite when it was appended. */
+/* The cache of one layer.  A key (value) is its e4m3 code times the scale of its page and head.
+ * Below a sequence's length value codes are finite; a key of NaN codes marks a token that was not
+ * finite when it was appended.  Slots past the length may hold anything. */
 typedef struct {
     void *k, *v;              /* e4m3 [num_pages][kv_heads][page_size][128], 128-byte aligned     */
     float *k_scale, *v_scale; /* f32 [num_pages][kv_heads], >= 0                                  */
@@ -90,7 +91,9 @@ MMRS_API int mmrs_paged_attend_status(const void *workspace);
  * with window > 0, of those only p - j < window and j < sinks (the first tokens stay visible).
  * out [total_q][query_heads][128] of `type` = softmax(scale q k) v; lse f32 [total_q][query_heads]
  * (or null) = ln sum exp(scale q k).  A row that sees nothing gives 0 and -infinity.  Statistics
- * and sums are f32; probabilities are rounded to f16 for the second product. */
+ * and sums are f32; probabilities are rounded to f16 for the second product, bf16 queries go to f16
+ * after an exact power-of-two scaling of their row, and value scales relative to the largest one met
+ * are rounded to f16 (exact for the powers of two that the append writes). */
 MMRS_API int mmrs_paged_attend(const MmrsPagedCache *cache, const MmrsPagedBatch *batch, const void *q,
                                int64_t q_stride, int type, int query_heads, float scale, int window, int sinks,
                                void *out, float *lse, void *workspace, size_t workspace_bytes, mmrs_stream_t stream);
