@@ -70,6 +70,33 @@ __device__ __forceinline__ void vf_load4(const T *row, int i, int n, float fill,
         for (int k = 0; k < 4; ++k) x[k] = i + k < n ? pg_to_float(row[i + k]) : fill;
     }
 }
+// 16 bytes at i (a multiple of their number of elements) of a row of n, as they are; -infinity past n.
+template <typename T>
+__device__ __forceinline__ uint4 vf_load16(const T *row, int i, int n) {
+    constexpr int kN = 16 / sizeof(T);
+    if (i + kN <= n && ((uintptr_t)(row + i) & 15) == 0) return *reinterpret_cast<const uint4 *>(row + i);
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if constexpr (sizeof(T) == 4) {
+            w[k] = i + k < n ? reinterpret_cast<const uint32_t *>(row)[i + k] : 0xff800000u;
+        } else {
+            constexpr uint32_t kNone = __is_same(T, __half) ? 0xfc00u : 0xff80u;
+            const uint16_t *r = reinterpret_cast<const uint16_t *>(row);
+            w[k] = (i + 2 * k < n ? r[i + 2 * k] : kNone) | (i + 2 * k + 1 < n ? r[i + 2 * k + 1] : kNone) << 16;
+        }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// The elements of a word: one, or two.
+__device__ __forceinline__ void vf_split(uint32_t w, float (&x)[1], const float *) { x[0] = __uint_as_float(w); }
+__device__ __forceinline__ void vf_split(uint32_t w, float (&x)[2], const __half *) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+    x[0] = f.x, x[1] = f.y;
+}
+__device__ __forceinline__ void vf_split(uint32_t w, float (&x)[2], const __nv_bfloat16 *) {
+    x[0] = __uint_as_float(w << 16), x[1] = __uint_as_float(w & 0xffff0000u);
+}
 // (m, s) of the warp's parts: one rescaling each, then plain sums.
 __device__ __forceinline__ void vf_join_warp(float &m, float &s, float c) {
     const float top = warp_max_butterfly(m);
@@ -137,7 +164,7 @@ __device__ __forceinline__ void vf_judge(const VfParams &p, int s, int row0, int
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kVfThreads, 4) verify_rows_kernel(const VfParams p) {
+__global__ void __launch_bounds__(kVfThreads, sizeof(T) == 4 ? 4 : 3) verify_rows_kernel(const VfParams p) {
     __shared__ float s_m[kVfWarps], s_s[kVfWarps];
     __shared__ unsigned long long s_b[kVfWarps];
     __shared__ int s_last;
@@ -147,10 +174,16 @@ __global__ void __launch_bounds__(kVfThreads, 4) verify_rows_kernel(const VfPara
     if (row >= p.total_rows) return;
     const T *l = static_cast<const T *>(p.logits) + (long)row * p.vocab;
     const int c0 = blockIdx.y * p.chunk, c1 = min(c0 + p.chunk, p.vocab);
-    float x[kVfGroups][4];
+    constexpr int kN = 16 / sizeof(T), kW = 4 / sizeof(T);  // elements of a read and of a word of it
+    uint32_t x[4 * kVfGroups];
+    auto load = [&](int i0) {
 #pragma unroll
-    for (int j = 0; j < kVfGroups; ++j)  // on the way while the row's sequence is looked up
-        vf_load4(l, c0 + (j * kVfThreads + threadIdx.x) * 4, c1, -INFINITY, x[j]);
+        for (int j = 0; j < kVfGroups; ++j) {
+            const uint4 r = vf_load16(l, i0 + (j * kVfThreads + (int)threadIdx.x) * kN, c1);
+            x[4 * j] = r.x, x[4 * j + 1] = r.y, x[4 * j + 2] = r.z, x[4 * j + 3] = r.w;
+        }
+    };
+    load(c0);  // on the way while the row's sequence is looked up
     int s = 0;
     for (int s0 = 0; s0 < p.num_seqs; s0 += 32)
         s += __popc(__ballot_sync(0xffffffffu, s0 + lane < p.num_seqs && p.cu[s0 + lane + 1] <= row));
@@ -163,27 +196,41 @@ __global__ void __launch_bounds__(kVfThreads, 4) verify_rows_kernel(const VfPara
     for (int i0 = c0;;) {
         float top = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < kVfGroups; ++j)
+        for (int j = 0; j < 4 * kVfGroups; ++j) {
+            float e[kW];
+            vf_split(x[j], e, (const T *)nullptr);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) top = fmaxf(top, x[j][k]);
+            for (int k = 0; k < kW; ++k) top = fmaxf(top, e[k]);
+            if constexpr (kW == 2) asm volatile("" : "+r"(x[j]));
+        }
         if (greedy) {
 #pragma unroll
-            for (int j = 0; j < kVfGroups; ++j)
+            for (int j = 0; j < 4 * kVfGroups; ++j) {
+                float e[kW];
+                vf_split(x[j], e, (const T *)nullptr);
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (x[j][k] > best) best = x[j][k], at = i0 + (j * kVfThreads + (int)threadIdx.x) * 4 + k;
+                for (int k = 0; k < kW; ++k)
+                    if (e[k] > best)
+                        best = e[k], at = i0 + ((j / 4) * kVfThreads + (int)threadIdx.x) * kN + (j % 4) * kW + k;
+            }
         }
+        // (the words are taken apart a second time: twice as many floats would not stay in registers)
+#pragma unroll
+        for (int j = 0; j < 4 * kVfGroups; ++j)
+            if constexpr (kW == 2) asm volatile("" : "+r"(x[j]));
         const float base = top == -INFINITY ? 0.0f : top;
         float part = 0.0f;
 #pragma unroll
-        for (int j = 0; j < kVfGroups; ++j)
+        for (int j = 0; j < 4 * kVfGroups; ++j) {
+            float e[kW];
+            vf_split(x[j], e, (const T *)nullptr);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) part += vf_exp2((x[j][k] - base) * c);  // an infinity leaves NaN here
+            for (int k = 0; k < kW; ++k) part += vf_exp2((e[k] - base) * c);  // an infinity leaves NaN here
+        }
         vf_join(m, sum, top, part, c);
-        i0 += kVfBlock;
+        i0 += kVfThreads * kVfGroups * kN;
         if (i0 >= c1) break;
-#pragma unroll
-        for (int j = 0; j < kVfGroups; ++j) vf_load4(l, i0 + (j * kVfThreads + threadIdx.x) * 4, c1, -INFINITY, x[j]);
+        load(i0);
     }
     unsigned long long key = at >= 0 ? lm_key(best, at) : 0;
     vf_join_warp(m, sum, c);
@@ -385,20 +432,21 @@ extern "C" int mmrs_verify_drafts(const void *logits, int logits_type, int vocab
     p.q = draft_probs, p.u = uniforms, p.noise = noise, p.temperature = temperature;
     p.tokens = tokens, p.accepted = accepted, p.logprobs = logprobs;
     // chunks of a row: of all numbers of them the one whose rounds of resident blocks (a block's beginning
-    // and end count as two reads of 8192 tokens) are the shortest in all, fewer chunks first
-    auto chunk_of = [&](long rows, int resident) {
-        const int most = (vocab + kVfBlock - 1) / kVfBlock;
+    // and end count as two reads of a block) are the shortest in all, fewer chunks first
+    auto chunk_of = [&](long rows, int resident, int block) {
+        const int most = (vocab + block - 1) / block;
         long best = -1;
         int chunk = 0;
         for (int n = 1; n <= kVfChunks && n <= most; ++n) {
             const int reads = (most + n - 1) / n;
             const long rounds = (rows * ((most + reads - 1) / reads) + 148L * resident - 1) / (148L * resident);
             const long cost = rounds * (reads + 2);
-            if (best < 0 || cost < best) best = cost, chunk = reads * kVfBlock;
+            if (best < 0 || cost < best) best = cost, chunk = reads * block;
         }
         return chunk;
     };
-    p.chunk = chunk_of(total_rows, 4), p.race_chunk = chunk_of(num_seqs, 2);
+    p.chunk = logits_type == MMRS_TYPE_F32 ? chunk_of(total_rows, 4, kVfBlock) : chunk_of(total_rows, 3, 2 * kVfBlock);
+    p.race_chunk = chunk_of(num_seqs, 2, kVfBlock);
     p.chunks = (vocab + p.chunk - 1) / p.chunk;
     p.race_chunks = (vocab + p.race_chunk - 1) / p.race_chunk;
     uint8_t *ws = static_cast<uint8_t *>(workspace);
