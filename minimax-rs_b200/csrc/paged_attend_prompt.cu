@@ -722,30 +722,63 @@ __device__ void pp_softmax(const PaParams &p, PpShared &sm, int u0, int u1, int 
             }
             named_sync(1, 256);
             if (sm.last) {
-#pragma unroll 1
-                for (int r = warp; r < s.rows; r += 8) {
-                    auto at = [&](int c) { return p.partials + ((size_t)c * 2 + (c == c0 ? 1 : 0)) * kPpSlotFloats; };
+                // a row's maximum and sum by one thread, then eight rows a warp at a time, their reads in
+                // flight together (the queries' tiles are free: every product of the piece has ended)
+                float *row_top = reinterpret_cast<float *>(sm.q), *row_inv = row_top + kPpRows;
+                auto part = [&](int c) { return p.partials + ((size_t)c * 2 + (c == c0 ? 1 : 0)) * kPpSlotFloats; };
+                auto where = [&](int r) {
+                    return (long)(s.seq.row0 + (s.row0 + r) / p.group) * p.query_heads + s.h * p.group + (s.row0 + r) % p.group;
+                };
+                if ((int)threadIdx.x < s.rows) {
+                    const int r = threadIdx.x;
                     float top = -INFINITY, l = 0.0f;
-                    for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, __ldcg(at(c) + (size_t)kPpRows * kPgDim + r));
-                    top = warp_max_butterfly(top);
-                    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+                    for (int c = c0; c <= c1; ++c) top = fmaxf(top, __ldcg(part(c) + (size_t)kPpRows * kPgDim + r));
 #pragma unroll 4
                     for (int c = c0; c <= c1; ++c) {
-                        const float *a = at(c);
-                        const float f = top == -INFINITY ? 1.0f : pa_exp2(__ldcg(a + (size_t)kPpRows * kPgDim + r) - top);
-                        const float4 x = __ldcg(reinterpret_cast<const float4 *>(a + (size_t)r * kPgDim) + lane);
-                        l += f * __ldcg(a + (size_t)kPpRows * (kPgDim + 1) + r);
-                        acc.x += f * x.x, acc.y += f * x.y, acc.z += f * x.z, acc.w += f * x.w;
+                        const float *a = part(c) + (size_t)kPpRows * kPgDim + r;
+                        l += (top == -INFINITY ? 1.0f : pa_exp2(__ldcg(a) - top)) * __ldcg(a + kPpRows);
                     }
-                    const long dst = (long)(s.seq.row0 + (s.row0 + r) / p.group) * p.query_heads + s.h * p.group +
-                                     (s.row0 + r) % p.group;
                     const bool none = top == -INFINITY && l == l;
-                    const float inv = none ? 0.0f : 1.0f / l;
-                    T *out = static_cast<T *>(p.out) + dst * kPgDim;
-                    reinterpret_cast<uint2 *>(out)[lane] =
-                        make_uint2(pg_pack2(acc.x * inv, acc.y * inv, out), pg_pack2(acc.z * inv, acc.w * inv, out));
-                    if (p.lse && lane == 0) p.lse[dst] = none ? -INFINITY : (top + log2f(l)) * kPaLn2;
+                    row_top[r] = top, row_inv[r] = none ? 0.0f : 1.0f / l;
+                    if (p.lse) p.lse[where(r)] = none ? -INFINITY : (top + log2f(l)) * kPaLn2;
                 }
+                named_sync(1, 256);
+                constexpr int kAt = 8;
+#pragma unroll 1
+                for (int r0 = warp * kAt; r0 < s.rows; r0 += 8 * kAt) {
+                    float4 acc[kAt];
+#pragma unroll
+                    for (int x = 0; x < kAt; ++x) acc[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+                    for (int c = c0; c <= c1; ++c) {
+                        const float *a = part(c);
+                        float4 v[kAt];
+                        float f[kAt];
+#pragma unroll
+                        for (int x = 0; x < kAt; ++x) {
+                            const int r = min(r0 + x, s.rows - 1);
+                            v[x] = __ldcg(reinterpret_cast<const float4 *>(a + (size_t)r * kPgDim) + lane);
+                            f[x] = __ldcg(a + (size_t)kPpRows * kPgDim + r);
+                        }
+#pragma unroll
+                        for (int x = 0; x < kAt; ++x) {
+                            const float top = row_top[min(r0 + x, s.rows - 1)];
+                            const float g = top == -INFINITY ? 1.0f : pa_exp2(f[x] - top);
+                            acc[x].x += g * v[x].x, acc[x].y += g * v[x].y, acc[x].z += g * v[x].z, acc[x].w += g * v[x].w;
+                        }
+                    }
+#pragma unroll
+                    for (int x = 0; x < kAt; ++x) {
+                        if (r0 + x >= s.rows) break;
+                        const float inv = row_inv[r0 + x];
+                        T *out = static_cast<T *>(p.out) + where(r0 + x) * kPgDim;
+                        reinterpret_cast<uint2 *>(out)[lane] =
+                            make_uint2(pg_pack2(acc[x].x * inv, acc[x].y * inv, out),
+                                       pg_pack2(acc[x].z * inv, acc[x].w * inv, out));
+                    }
+                }
+                named_sync(1, 256);  // the next piece's queries go where the rows' maxima are
                 if (threadIdx.x == 0) p.counters[c0] = 0u;
             }
         }
