@@ -162,28 +162,17 @@ __device__ __forceinline__ uint64_t pp_exp2_fma(uint64_t x) {
 }
 __device__ __forceinline__ void pp_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// A row of S with -infinity where the row does not see the column: x > at, with a window (at - x >=
-// window and x >= first), or a group whose page holds nothing.  A pass of its own, so that the loops
-// over S stay short enough for the instruction cache (masks unrolled there cost more than they do).
-__device__ __forceinline__ void pp_mask(uint32_t ts, int at, int window, int first, const float *ks) {
-    const int gone = window > 0 ? at - window : -1, seen = window > 0 ? first : 0;
-#pragma unroll 1
-    for (int c = 0; c < 2; ++c) {
-        float v[32];
-        pp_ld32(ts + 32 * c, v);
-        const bool none0 = ks[2 * c] < 0.0f, none1 = ks[2 * c + 1] < 0.0f;
-        pp_wait_ld(v);
-        uint32_t w[2][16];
-#pragma unroll
-        for (int x = 0; x < 32; ++x) {
-            const int y = 32 * c + x;
-            const bool hide = y > at || (y <= gone && y >= seen) || (x < 16 ? none0 : none1);
-            w[x >> 4][x & 15] = __float_as_uint(hide ? -INFINITY : v[x]);
-        }
-        pp_st16(ts + 32 * c, w[0]);
-        pp_st16(ts + 32 * c + 16, w[1]);
-    }
-    pp_wait_st();
+// The columns of a 64-column half that a row sees, as bits: x <= at, with a window (x > at - window or
+// x < first), and the groups of 16 whose page holds something.
+__device__ __forceinline__ uint64_t pp_upto(int n) { return n < 0 ? 0ull : n >= 63 ? ~0ull : (2ull << n) - 1; }
+__device__ __forceinline__ uint64_t pp_sees(int at, int window, int first, const float4 &ks) {
+    uint64_t see = pp_upto(at);
+    if (window > 0) see &= ~pp_upto(at - window) | pp_upto(first - 1);
+    if (ks.x < 0.0f) see &= ~0xffffull;
+    if (ks.y < 0.0f) see &= ~(0xffffull << 16);
+    if (ks.z < 0.0f) see &= ~(0xffffull << 32);
+    if (ks.w < 0.0f) see &= ~(0xffffull << 48);
+    return see;
 }
 
 // A row of O times f.
@@ -522,36 +511,50 @@ __device__ void pp_products(const PaParams &p, PpShared &sm, int u0, int u1) {
 }
 
 // ---- warps 0-7: softmax and epilogue ----------------------------------------------------------
+// A warp's 32 rows of queries, from row r0 of the sequence's on (none past `last`), to the tile's rows
+// from row0 on; the factor of the row of this lane.  A lane takes row lane & 7 of each group of eight
+// and 16-byte pieces (lane >> 3) + 4 i: a read covers 64 bytes of eight rows, a write every bank once.
 template <typename T>
-__device__ __forceinline__ float pp_load_q(const PaParams &p, const PpSeg &s, int r, uint8_t *tile, int row) {
-    uint4 f[16];
-    const T *q = static_cast<const T *>(p.q) + (long)(s.seq.row0 + r / p.group) * p.q_stride +
-                 (s.h * p.group + r % p.group) * kPgDim;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) f[i] = reinterpret_cast<const uint4 *>(q)[i];
-    uint32_t *w = reinterpret_cast<uint32_t *>(f);
-    float up = 1.0f;
-    if constexpr (!__is_same(T, __half)) {
-        // to f16 with the row's largest value moved to [2^14, 2^15): exact but for values 2^-38 of it
-        // and less
-        float amax = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 64; ++i)
-            amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
-        const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127 - 14, -120), 120);
-        const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-        up = __uint_as_float((uint32_t)(127 + e) << 23);
-#pragma unroll
-        for (int i = 0; i < 64; ++i)
-            w[i] = pg_pack2(__uint_as_float(w[i] << 16) * down, __uint_as_float(w[i] & 0xffff0000u) * down,
-                            (const __half *)nullptr);
-    }
+__device__ __forceinline__ float pp_load_q(const PaParams &p, const PpSeg &s, int r0, int last, uint8_t *tile, int row0) {
+    const int lane = threadIdx.x & 31;
     const uint32_t sign = p.scale_log2 < 0.0f ? 0x80008000u : 0u;  // the columns' factors stay >= 0
-    uint8_t *at = tile + (row >> 3) * 128 + (row & 7) * 16;
+    uint4 f[4][4];
+    float up = 1.0f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-        *reinterpret_cast<uint4 *>(at + i * kPpSlice) =
-            make_uint4(f[i].x ^ sign, f[i].y ^ sign, f[i].z ^ sign, f[i].w ^ sign);
+    for (int g = 0; g < 4; ++g) {
+        const int r = r0 + 8 * g + (lane & 7);
+        const T *q = static_cast<const T *>(p.q) + (long)(s.seq.row0 + r / p.group) * p.q_stride +
+                     (s.h * p.group + r % p.group) * kPgDim + 8 * (lane >> 3);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            f[g][i] = r <= last ? *reinterpret_cast<const uint4 *>(q + 32 * i) : make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        uint32_t *w = reinterpret_cast<uint32_t *>(f[g]);
+        if constexpr (!__is_same(T, __half)) {
+            // to f16 with the row's largest value moved to [2^14, 2^15): exact but for values 2^-38 of it
+            // and less
+            float amax = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(w[i] << 16)), fabsf(__uint_as_float(w[i] & 0xffff0000u))));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 8));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 16));
+            const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127 - 14, -120), 120);
+            const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+            if (g == lane >> 3) up = __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                w[i] = pg_pack2(__uint_as_float(w[i] << 16) * down, __uint_as_float(w[i] & 0xffff0000u) * down,
+                                (const __half *)nullptr);
+        }
+        uint8_t *at = tile + ((row0 >> 3) + g) * 128 + (lane & 7) * 16 + (lane >> 3) * kPpSlice;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<uint4 *>(at + 4 * i * kPpSlice) =
+                make_uint4(f[g][i].x ^ sign, f[g][i].y ^ sign, f[g][i].z ^ sign, f[g][i].w ^ sign);
+    }
     return up * fabsf(p.scale_log2);
 }
 
@@ -584,7 +587,7 @@ __device__ void pp_softmax(const PaParams &p, PpShared &sm, int u0, int u1, int 
             const bool live = r < s.rows, warp_live = i * 128 + (warp & 3) * 32 < s.rows;
             const int pos = live ? s.seq.pos0 + (s.row0 + r) / p.group : -1;
             float m = -INFINITY, l = 0.0f, factor = 0.0f, vref = 1.0f;
-            if (live) factor = pp_load_q<T>(p, s, s.row0 + r, sm.q[i], row);
+            factor = pp_load_q<T>(p, s, s.row0 + r - lane, s.row0 + s.rows - 1, sm.q[i], row - lane);
             fence_proxy_async_smem();
             tc_fence_before();
             __syncwarp();
@@ -613,13 +616,18 @@ __device__ void pp_softmax(const PaParams &p, PpShared &sm, int u0, int u1, int 
                                            !(fminf(fminf(ks.x, ks.y), fminf(ks.z, ks.w)) < 0.0f);
                     pp_wait_ld(v[0]);
                     pp_hold32(v[1]);
+                    bool any = true;
                     if (!__all_sync(0xffffffffu, whole)) {
-                        pp_mask(tsh, pos - key0, p.window, p.sinks - key0, sc.k + 4 * h);
-                        pp_ld32(tsh, v[0]);
-                        pp_ld32(tsh + 32, v[1]);
-                        pp_wait_ld(v[0]);
-                        pp_hold32(v[1]);
+                        const uint64_t see = pp_sees(pos - key0, p.window, p.sinks - key0, ks);
+                        any = __any_sync(0xffffffffu, see != 0);
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            const uint32_t bits = (uint32_t)(see >> 32 * c);
+#pragma unroll
+                            for (int x = 0; x < 32; ++x) v[c][x] = bits >> x & 1 ? v[c][x] : -INFINITY;
+                        }
                     }
+                    if (any) {
                     // a column's factor: never 0, so that a masked score's -infinity stays one
                     const float col[4] = {fmaxf(ks.x * factor, 1e-35f), fmaxf(ks.y * factor, 1e-35f),
                                           fmaxf(ks.z * factor, 1e-35f), fmaxf(ks.w * factor, 1e-35f)};
@@ -632,10 +640,8 @@ __device__ void pp_softmax(const PaParams &p, PpShared &sm, int u0, int u1, int 
                         for (int c = 1; c < 8; ++c) mx = fmaxf(mx, x[c]), my = fmaxf(my, x[8 + c]);
                         top = fmaxf(top, fmaxf(mx, my) * col[g]);
                     }
-                    const bool grows = top > m + kPpLazy || (m == -INFINITY && top != -INFINITY);
-                    if (y == 0) {
-                        m = top;
-                    } else if (__any_sync(0xffffffffu, grows)) {
+                    if (m == -INFINITY) m = top;  // (O and l are zero: there is nothing to scale)
+                    if (__any_sync(0xffffffffu, top > m + kPpLazy)) {
                         const float now = fmaxf(m, top), f = now == -INFINITY ? 1.0f : pa_exp2(m - now);
                         m = now;
                         l *= f;
@@ -674,6 +680,11 @@ __device__ void pp_softmax(const PaParams &p, PpShared &sm, int u0, int u1, int 
                     float s0, s1;
                     pp_split(sum, s0, s1);
                     l += s0 + s1;
+                    } else {  // no row of the warp sees any of it
+                        const uint32_t zero[16] = {};
+                        pp_st16(tsh, zero);
+                        pp_st16(tsh + 16, zero);
+                    }
                     pp_wait_st();
                     tc_fence_before();
                 }
