@@ -48,6 +48,7 @@ struct alignas(16) PpScale {  // of the eight 16-position groups of a tile
 };
 struct PpShared {
     uint8_t q[2][kPpTile], k[kPpStages][kPpTile], v[kPpStages][kPpTile];
+    float row_top[kPpRows], row_inv[kPpRows];  // of an item's rows while its pieces are joined
     PpScale sc[kPpScales];
     float vmax[4];
     int prefix[kPaMaxSeqs + 1];
@@ -282,6 +283,21 @@ __device__ void pp_seek(const PaParams &p, const PpShared &sm, int u, int end, i
     s.row0 = rt * kPpRows;
     s.rows = min(kPpRows, s.seq.count * p.group - s.row0);
 }
+// The piece after s, which ends an item at unit u (whole warp): the lookup of pp_seek, some 2500 cycles,
+// only where a new sequence begins.
+__device__ void pp_next(const PaParams &p, const PpShared &sm, int u, int end, int lane, PpSeg &s) {
+    int rt = s.row0 / kPpRows + 1, h = s.h;
+    if (rt * kPpRows >= s.seq.count * p.group) rt = 0, ++h;
+    if (h >= p.c.kv_heads) {
+        pp_seek(p, sm, u, end, lane, s);
+        return;
+    }
+    s.h = h, s.off = 0;
+    s.nb = pp_tiles(p, s.seq, rt, s.span);
+    s.n = min(s.nb, end - u);
+    s.row0 = rt * kPpRows;
+    s.rows = min(kPpRows, s.seq.count * p.group - s.row0);
+}
 
 // A read that leaves the L1 alone.
 __device__ __forceinline__ uint4 pp_ldg(const uint8_t *at) {
@@ -321,10 +337,11 @@ __device__ void pp_convert(const PaParams &p, PpShared &sm, int u0, int u1) {
     const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) - kPpConvWarp0;
     int tile = 0;
     bool ok = true;  // after a failed wait only the barriers among these warps go on
+    PpSeg s;
 #pragma unroll 1
     for (int u = u0; u < u1;) {
-        PpSeg s;
-        pp_seek(p, sm, u, u1, lane, s);
+        if (u == u0) pp_seek(p, sm, u, u1, lane, s);
+        else pp_next(p, sm, u, u1, lane, s);
         const int ps = p.c.page_size;
         // the pages and scales of this warp's two 16-position groups in 16 tiles, one a lane
         int pid = -1;
@@ -344,7 +361,7 @@ __device__ void pp_convert(const PaParams &p, PpShared &sm, int u0, int u1) {
         };
         float vref = 0.0f;
 #pragma unroll 1
-        for (int base = 0; base < s.n; base += 16) {
+        for (int base = (s.n - 1) & ~15; base >= 0; base -= 16) {  // the first sixteen last: they come next
             fetch(base);
             vref = fmaxf(vref, vs);
         }
@@ -377,7 +394,6 @@ __device__ void pp_convert(const PaParams &p, PpShared &sm, int u0, int u1) {
                 if (left[g] > 8 * u) r[it] = pp_ldg(base + at[g] + u * 8 * kPgDim + (it & 1) * 64);
             }
         };
-        fetch(0);
         place(0);
         load(p.c.k, kr);
         load(p.c.v, vr);
@@ -460,10 +476,11 @@ __device__ void pp_products(const PaParams &p, PpShared &sm, int u0, int u1) {
     };
     auto test = [&](uint64_t *bar, int use) { return mbar_test_wait(bar, (uint32_t)use & 1); };
     int tile = 0, pieces = 0, used = 0;  // tiles of the CTA so far; pieces and tiles of this row tile
+    PpSeg s;
 #pragma unroll 1
     for (int u = u0; ok && u < u1;) {
-        PpSeg s;
-        pp_seek(p, sm, u, u1, lane, s);
+        if (u == u0) pp_seek(p, sm, u, u1, lane, s);
+        else pp_next(p, sm, u, u1, lane, s);
         const int n = __shfl_sync(0xffffffffu, s.n, 0);
         if (i == 0 || s.rows > 128) {
             wait(&sm.k_full[tile % kPpStages], tile / kPpStages);
@@ -575,23 +592,29 @@ __device__ void pp_softmax(const PaParams &p, PpShared &sm, int u0, int u1, int 
     const uint32_t ts = sm.tmem + lanes + kColS + 128 * i, to = sm.tmem + lanes + kColO + 128 * i;
     int tile = 0, used = 0;
     bool ok = true;  // after a failed wait only the barriers among these warps go on
+    float factor = 0.0f;
+    // a piece's queries
+    auto queries = [&](const PpSeg &s) {
+        if (i == 1 && s.rows <= 128) return;
+        factor = pp_load_q<T>(p, s, s.row0 + i * 128 + row - lane, s.row0 + s.rows - 1, sm.q[i], row - lane);
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.q_full[i]);
+    };
+    PpSeg s;
+    pp_seek(p, sm, u0, u1, lane, s);
+    queries(s);
 #pragma unroll 1
     for (int u = u0; u < u1;) {
-        PpSeg s;
-        pp_seek(p, sm, u, u1, lane, s);
         const int end = u - s.off + s.nb, c0 = (u - s.off) / share, c1 = (end - 1) / share;
         float *slot = p.partials + ((size_t)blockIdx.x * 2 + ((int)blockIdx.x == c0 ? 1 : 0)) * kPpSlotFloats;
-        const bool two = s.rows > 128;
-        if (ok && (i == 0 || two)) {
-            const int r = i * 128 + row;  // of the item
-            const bool live = r < s.rows, warp_live = i * 128 + (warp & 3) * 32 < s.rows;
-            const int pos = live ? s.seq.pos0 + (s.row0 + r) / p.group : -1;
-            float m = -INFINITY, l = 0.0f, factor = 0.0f, vref = 1.0f;
-            factor = pp_load_q<T>(p, s, s.row0 + r - lane, s.row0 + s.rows - 1, sm.q[i], row - lane);
-            fence_proxy_async_smem();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sm.q_full[i]);
+        const bool mine = i == 0 || s.rows > 128;
+        const int r = i * 128 + row;  // of the item
+        const bool live = r < s.rows, warp_live = i * 128 + (warp & 3) * 32 < s.rows;
+        const int pos = live ? s.seq.pos0 + (s.row0 + r) / p.group : -1;
+        float m = -INFINITY, l = 0.0f, vref = 1.0f;
+        if (ok && mine) {
 #pragma unroll 1
             for (int y = 0; y < 2 * s.n; ++y) {
                 const int j = y >> 1, h = y & 1, at = tile + j;
@@ -691,7 +714,16 @@ __device__ void pp_softmax(const PaParams &p, PpShared &sm, int u0, int u1, int 
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sm.p_full[i][h]);
             }
-            ok = ok && pp_wait_warp(&sm.o_done[i][1], (uint32_t)(used + s.n - 1) & 1, sm, p);
+        }
+        // The next piece's queries, so that its first scores are under way while this one's O is read: the
+        // scores that used these queries have all been here.
+        PpSeg next = s;
+        if (ok && u + s.n < u1) {
+            pp_next(p, sm, u + s.n, u1, lane, next);
+            queries(next);
+        }
+        if (ok && mine) {
+            ok = pp_wait_warp(&sm.o_done[i][1], (uint32_t)(used + s.n - 1) & 1, sm, p);
             tc_fence_after();
             used += s.n;
             if (ok && warp_live) {
@@ -734,8 +766,7 @@ __device__ void pp_softmax(const PaParams &p, PpShared &sm, int u0, int u1, int 
             named_sync(1, 256);
             if (sm.last) {
                 // a row's maximum and sum by one thread, then eight rows a warp at a time, their reads in
-                // flight together (the queries' tiles are free: every product of the piece has ended)
-                float *row_top = reinterpret_cast<float *>(sm.q), *row_inv = row_top + kPpRows;
+                // flight together
                 auto part = [&](int c) { return p.partials + ((size_t)c * 2 + (c == c0 ? 1 : 0)) * kPpSlotFloats; };
                 auto where = [&](int r) {
                     return (long)(s.seq.row0 + (s.row0 + r) / p.group) * p.query_heads + s.h * p.group + (s.row0 + r) % p.group;
@@ -751,7 +782,7 @@ __device__ void pp_softmax(const PaParams &p, PpShared &sm, int u0, int u1, int 
                         l += (top == -INFINITY ? 1.0f : pa_exp2(__ldcg(a) - top)) * __ldcg(a + kPpRows);
                     }
                     const bool none = top == -INFINITY && l == l;
-                    row_top[r] = top, row_inv[r] = none ? 0.0f : 1.0f / l;
+                    sm.row_top[r] = top, sm.row_inv[r] = none ? 0.0f : 1.0f / l;
                     if (p.lse) p.lse[where(r)] = none ? -INFINITY : (top + log2f(l)) * kPaLn2;
                 }
                 named_sync(1, 256);
@@ -774,7 +805,7 @@ __device__ void pp_softmax(const PaParams &p, PpShared &sm, int u0, int u1, int 
                         }
 #pragma unroll
                         for (int x = 0; x < kAt; ++x) {
-                            const float top = row_top[min(r0 + x, s.rows - 1)];
+                            const float top = sm.row_top[min(r0 + x, s.rows - 1)];
                             const float g = top == -INFINITY ? 1.0f : pa_exp2(f[x] - top);
                             acc[x].x += g * v[x].x, acc[x].y += g * v[x].y, acc[x].z += g * v[x].z, acc[x].w += g * v[x].w;
                         }
@@ -782,19 +813,19 @@ __device__ void pp_softmax(const PaParams &p, PpShared &sm, int u0, int u1, int 
 #pragma unroll
                     for (int x = 0; x < kAt; ++x) {
                         if (r0 + x >= s.rows) break;
-                        const float inv = row_inv[r0 + x];
+                        const float inv = sm.row_inv[r0 + x];
                         T *out = static_cast<T *>(p.out) + where(r0 + x) * kPgDim;
                         reinterpret_cast<uint2 *>(out)[lane] =
                             make_uint2(pg_pack2(acc[x].x * inv, acc[x].y * inv, out),
                                        pg_pack2(acc[x].z * inv, acc[x].w * inv, out));
                     }
                 }
-                named_sync(1, 256);  // the next piece's queries go where the rows' maxima are
                 if (threadIdx.x == 0) p.counters[c0] = 0u;
             }
         }
         tile += s.n;
         u += s.n;
+        s = next;
     }
 }
 
