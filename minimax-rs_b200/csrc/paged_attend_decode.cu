@@ -1,4 +1,5 @@
-// Paged attention for few rows: single tokens and drafted tokens (at most kPaFewRows rows a KV head).
+// Paged attention for few rows: single tokens and drafted tokens (at most kPaFewRows rows a KV head, in
+// groups of up to 32, an item each; a kernel for 8, 16, 24 and 32 rows).
 //
 // Each K / V code is read once and used for all rows of its KV head, so the kernel is bound by HBM:
 // 256 bytes a position and head.  The products run on mma.sync with the operands turned round, S^T =
@@ -18,6 +19,13 @@
 // with a ring of TMA copies of its own, its own running maximum and sum, and no barrier until the end
 // of a (sequence, head).  Where that end lies in another CTA, the CTAs' partial results go through
 // the workspace and the last to arrive joins them in order.
+//
+// Measured (48 + 8 heads): one token over 196608 positions 74 us (403 MB, 5.4 TB/s, 0.83 of a plain
+// copy's; the same ring without the arithmetic takes 67); one token over 4096 positions 11.2 us in a
+// captured graph (a chain of latencies: launch, lookups, first tiles, joins); 64 sequences of 1001 to 8192
+// positions and 5 drafted tokens (30 rows) 250 us (612 MB, 2.5 TB/s): eight warps of 255 registers, each
+// with a chain of 128 products, 512 codes to turn and 32 exponentials a lane in a step, leave the
+// issue slots two thirds empty and memory at 0.37.  Twelve warps of 168 registers, two a step: 475 us.
 #include "paged_attend.cuh"
 
 #include <algorithm>
