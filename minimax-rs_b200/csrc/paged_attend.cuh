@@ -11,10 +11,10 @@ namespace mmrs {
 
 constexpr int kPaMaxSeqs = MMRS_PAGED_MAX_SEQS;
 constexpr int kPaDecodeRows = 32;  // rows of an item of the decode kernel, at most
-// Rows of a KV head up to which a sequence is the decode kernel's: it takes 250 us for 30 rows of 64
-// sequences (300000 positions, 8 heads), with each further group of 32 as long again, the prompt kernel
-// 880 us for any number up to 128.
-constexpr int kPaFewRows = 96;
+// Rows of a KV head up to which a sequence is the decode kernel's: 64 sequences (300000 positions, 8
+// heads) take it 250 us with 30 rows, 369 with 48, 480 with 54, 723 with 96, and the prompt kernel 340 to
+// 350 with any number up to 128; 4 sequences 38 us with 48 rows, 46 with 54, 60 with 96, and 50 to 55.
+constexpr int kPaFewRows = 48;
 constexpr float kPaLog2e = 1.4426950408889634f;
 constexpr float kPaLn2 = 0.6931471805599453f;
 constexpr uint64_t kPaTimeoutNs = 2000000000ull;

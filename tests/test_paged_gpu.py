@@ -52,10 +52,10 @@ def test_attend_drafts(pkg, dev, group, kv, seqs):
 
 
 @pytest.mark.parametrize("page", [16, 128])
-@pytest.mark.parametrize("group,new", [(6, 6), (6, 11), (6, 16), (16, 3), (16, 6), (1, 33), (1, 64), (1, 65), (1, 96),
-                                       (1, 97), (5, 19), (5, 20)])
+@pytest.mark.parametrize("group,new", [(6, 6), (6, 8), (6, 9), (6, 11), (6, 16), (16, 3), (16, 4), (16, 6), (1, 33),
+                                       (1, 48), (1, 49), (1, 64), (1, 65), (1, 96), (1, 97), (5, 9), (5, 10), (5, 20)])
 def test_attend_rows_around_the_kernels_bounds(pkg, dev, page, group, new):
-    """33 to 100 rows a KV head: groups of 32 of the one kernel up to 96, the other kernel from there."""
+    """33 to 100 rows a KV head: two groups of the one kernel up to 48, one or both tiles of the other from there."""
     c = Case([(new, 400), (new, new), (1, 77), (new - 1, 1000)], page, 2, seed=page + new)
     c.spoil_unused()
     check_attend(pkg, dev, c, 2 * group, torch.float16)
