@@ -11,7 +11,7 @@
 //                         the sequence's last block to finish joins the chunks' winners.  It starts
 //                         while the first kernel drains, with its noise on the way.
 // A block reads 64 bytes a thread at once and keeps them in registers: 8192 f32 or 16384 16-bit tokens
-// (8192 of 16 bits: 33 ragged rows 39 us instead of 37, 320 rows of f16 86 instead of 80).  A row is cut
+// (8192 of 16 bits: 33 ragged sequences 39 us instead of 37, 320 rows of f16 86 instead of 76).  A row is cut
 // into the number of chunks whose rounds of resident blocks are the shortest.
 // Measured (200064 tokens, with the draft model's probabilities unless said): 5 rows of f32 12.1 us in a
 // captured graph (two launches and their dependent reads; the bytes alone would take 0.9); 320 rows of
@@ -19,6 +19,8 @@
 // probabilities 37 us (floor 12: rounds of blocks that wait for their own reads).
 #include <cuda_runtime.h>
 #include <math.h>
+
+#include <type_traits>
 
 #include "../../include/minimax_sample.h"
 #include "paged.cuh"
@@ -101,6 +103,24 @@ __device__ __forceinline__ void vf_split(uint32_t w, float (&x)[2], const __half
 }
 __device__ __forceinline__ void vf_split(uint32_t w, float (&x)[2], const __nv_bfloat16 *) {
     x[0] = __uint_as_float(w << 16), x[1] = __uint_as_float(w & 0xffff0000u);
+}
+// The largest element of the words (NaN aside).
+template <int kN>
+__device__ __forceinline__ float vf_top(const uint32_t (&x)[kN], const float *) {
+    float top = __uint_as_float(x[0]);
+#pragma unroll
+    for (int j = 1; j < kN; ++j) top = fmaxf(top, __uint_as_float(x[j]));
+    return fmaxf(top, -INFINITY);
+}
+template <int kN, typename T>
+__device__ __forceinline__ float vf_top(const uint32_t (&x)[kN], const T *t) {
+    using T2 = std::conditional_t<__is_same(T, __half), __half2, __nv_bfloat162>;
+    T2 top = *reinterpret_cast<const T2 *>(&x[0]);
+#pragma unroll
+    for (int j = 1; j < kN; ++j) top = __hmax2(top, *reinterpret_cast<const T2 *>(&x[j]));
+    float e[2];
+    vf_split(*reinterpret_cast<const uint32_t *>(&top), e, t);
+    return fmaxf(fmaxf(e[0], e[1]), -INFINITY);
 }
 // (m, s) of the warp's parts: one rescaling each, then plain sums.
 __device__ __forceinline__ void vf_join_warp(float &m, float &s, float c) {
@@ -199,15 +219,7 @@ __global__ void __launch_bounds__(kVfThreads, sizeof(T) == 4 ? 4 : 3) verify_row
     float m = -INFINITY, sum = 0.0f, best = -INFINITY;
     int at = -1;
     for (int i0 = c0;;) {
-        float top = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < 4 * kVfGroups; ++j) {
-            float e[kW];
-            vf_split(x[j], e, (const T *)nullptr);
-#pragma unroll
-            for (int k = 0; k < kW; ++k) top = fmaxf(top, e[k]);
-            if constexpr (kW == 2) asm volatile("" : "+r"(x[j]));
-        }
+        const float top = vf_top(x, (const T *)nullptr);
         if (greedy) {
 #pragma unroll
             for (int j = 0; j < 4 * kVfGroups; ++j) {
