@@ -451,7 +451,7 @@ def _raw_stream(stream, t) -> int:
     if stream is not None:
         return stream.cuda_stream
     import torch
-    return torch._C._cuda_getCurrentRawStream(t.device.index)
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def _on_stream(stream):
@@ -470,15 +470,19 @@ def _same_device(dev: int, *tensors) -> None:
             raise MoeError(MMRS_ERR_ARG, f"tensors on GPU {dev}")
 
 
-def _token_stride(t, heads: int, what: str) -> int:
-    """Elements between the token rows of t [tokens][heads][128], whose rows are contiguous."""
-    shape, stride = t.shape, t.stride()
-    n = shape[0]
+def _tokens(t, heads, what: str):
+    """(tokens, heads, elements between token rows) of t [tokens][heads][128], whose rows are contiguous;
+    heads None: as many as t has."""
+    try:
+        n, h, d = t.shape
+        row, head, one = t.stride()
+    except ValueError:
+        n, h, d, row, head, one = 1, -1, 0, 0, 0, 0
     if n == 0:
-        return heads * HEAD_DIM
-    if len(shape) != 3 or shape[1] != heads or shape[2] != HEAD_DIM or stride[2] != 1 or (heads > 1 and stride[1] != HEAD_DIM):
-        raise MoeError(MMRS_ERR_ARG, f"{what}: [tokens][{heads}][{HEAD_DIM}], heads side by side")
-    return stride[0] if n > 1 else max(stride[0], heads * HEAD_DIM)
+        return 0, h, h * HEAD_DIM
+    if d != HEAD_DIM or one != 1 or h != (heads or h) or h < 1 or (head != HEAD_DIM and h > 1):
+        raise MoeError(MMRS_ERR_ARG, f"{what}: [tokens][{heads or 'heads'}][{HEAD_DIM}], heads side by side")
+    return n, h, row if n > 1 else max(row, h * HEAD_DIM)
 
 
 class PagedBatch:
@@ -555,33 +559,35 @@ class PagedKvCache:
         """Writes the rotated k and v [tokens][kv_heads][128] (f32, f16 or bf16; row slices of one wider
         tensor will do) at the batch's positions; returns the rotated q (bf16 for bf16 queries, else
         f16; None for q None).  rope_cos / rope_sin: f32 [positions][rope_dim / 2]."""
-        n, dtype = k.shape[0], k.dtype
+        dtype = k.dtype
         code = _type_code(dtype)
         _same_device(self.device_index, batch.t[1], q, k, v, rope_cos, rope_sin, q_out)
-        if v.shape[0] != n or v.dtype != dtype or (q is not None and (q.shape[0] != n or q.dtype != dtype)):
+        n, _, k_stride = _tokens(k, self.kv_heads, "k")
+        v_n, _, v_stride = _tokens(v, self.kv_heads, "v")
+        if v_n != n or v.dtype is not dtype:
             raise MoeError(MMRS_ERR_ARG, "q, k, v: the same tokens, one element type")
-        rope = rope_cos.shape
-        if (rope != rope_sin.shape or _type_code(rope_cos.dtype) or _type_code(rope_sin.dtype) or
+        rope, f32 = rope_cos.shape, self.k_scale.dtype
+        if (len(rope) != 2 or rope != rope_sin.shape or rope_cos.dtype is not f32 or rope_sin.dtype is not f32 or
                 not rope_cos.is_contiguous() or not rope_sin.is_contiguous()):
             raise MoeError(MMRS_ERR_ARG, "rope_cos, rope_sin: f32 [positions][rope_dim / 2]")
         heads = q_stride = out_code = 0
         q_ptr = out_ptr = None
         if q is not None:
-            heads = q.shape[1]
-            q_stride = _token_stride(q, heads, "q")
+            q_n, heads, q_stride = _tokens(q, None, "q")
+            if q_n != n or q.dtype is not dtype:
+                raise MoeError(MMRS_ERR_ARG, "q, k, v: the same tokens, one element type")
             if q_out is None:
                 import torch
                 with _on_stream(stream):
                     q_out = torch.empty(n, heads, HEAD_DIM, device=q.device,
                                         dtype=torch.bfloat16 if code == 2 else torch.float16)
-            if q_out.shape != q.shape or not q_out.is_contiguous():
+            elif q_out.shape != q.shape or not q_out.is_contiguous():
                 raise MoeError(MMRS_ERR_ARG, "q_out: contiguous, shaped as q")
             out_code = _type_code(q_out.dtype)
             q_ptr, out_ptr = q.data_ptr(), q_out.data_ptr()
         rc = lib().mmrs_paged_append(self._ref, batch.bind(self, n), q_ptr, k.data_ptr(), v.data_ptr(), q_stride,
-                                     _token_stride(k, self.kv_heads, "k"), _token_stride(v, self.kv_heads, "v"), code,
-                                     heads, rope_cos.data_ptr(), rope_sin.data_ptr(), 2 * rope[1], rope[0], out_ptr,
-                                     out_code, _raw_stream(stream, k))
+                                     k_stride, v_stride, code, heads, rope_cos.data_ptr(), rope_sin.data_ptr(),
+                                     2 * rope[1], rope[0], out_ptr, out_code, _raw_stream(stream, k))
         if rc:
             raise MoeError(rc, "mmrs_paged_append")
         return q_out
@@ -612,8 +618,7 @@ class PagedKvCache:
         each token's own; with window > 0 only the last `window` of them and the first `sinks`.  lse
         f32 [tokens][heads] is filled when given.  scale: 1 / sqrt(128) unless given.  The calls of
         one cache share a workspace: keep them on one stream."""
-        n, heads = q.shape[:2]
-        stride = _token_stride(q, heads, "q")
+        n, heads, stride = _tokens(q, None, "q")
         _same_device(self.device_index, batch.t[1], q, out, lse)
         if out is None:
             import torch
