@@ -13,6 +13,22 @@ namespace mmrs {
 
 constexpr int kPgDim = MMRS_PAGED_HEAD_DIM;
 
+// Launches a kernel that may start while the one before it in the stream ends: its own launch and
+// the setting up of barriers are then out of the way (one token over 4096 positions, call after call:
+// 13.3 -> 11.7 us; 48 windowed tokens 26.7 -> 24.7).  Each of these kernels waits (grid_dependency_wait)
+// before it touches global memory.  The prompt kernel is launched plainly: with this it was slower
+// (windowed prompts 165 -> 173 us).
+template <typename... P>
+int pg_launch(void (*kernel)(P...), unsigned grid, int threads, size_t smem, cudaStream_t s, const P &...args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid), cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = smem, cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr, cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? MMRS_OK : MMRS_ERR_LAUNCH;
+}
+
 // Element access by type: four (or eight) consecutive elements as f32.
 __device__ __forceinline__ void pg_load4(const float *p, float (&x)[4]) {
     const float4 v = *reinterpret_cast<const float4 *>(p);

@@ -14,6 +14,7 @@
 // registers, the others come from L2 again, which was faster than holding them all (128 registers,
 // 124-273 us) or none (129 us): 12390 tokens of f32, 48 + 8 heads, 587 MB in 107 us (5.5 TB/s).
 #include "paged.cuh"
+#include "tma.cuh"
 
 namespace mmrs {
 namespace {
@@ -263,6 +264,8 @@ __device__ void ap_rotate_row(const ApParams &p, int row) {
 
 template <typename T, typename O>
 __global__ void __launch_bounds__(kApThreads, kApResident) paged_append_kernel(const __grid_constant__ ApParams p) {
+    launch_dependents();
+    grid_dependency_wait();
     if ((int)blockIdx.x < p.kv_units)
         ap_store_run<T>(p, blockIdx.x);
     else
@@ -273,8 +276,7 @@ template <typename T, typename O>
 int ap_launch(const ApParams &p, cudaStream_t s) {
     const long grid = (long)p.kv_units + (p.q ? p.b.total_q : 0);
     if (grid > 0x7fffffffL) return MMRS_ERR_UNSUPPORTED;
-    paged_append_kernel<T, O><<<(unsigned)grid, kApThreads, 0, s>>>(p);
-    return cudaGetLastError() == cudaSuccess ? MMRS_OK : MMRS_ERR_LAUNCH;
+    return pg_launch(paged_append_kernel<T, O>, (unsigned)grid, kApThreads, 0, s, p);
 }
 
 }  // namespace

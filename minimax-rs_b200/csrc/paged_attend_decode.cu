@@ -172,11 +172,13 @@ struct PdKernel {
 
     static __device__ void run(const PaParams &p, const CUtensorMap *kmap, const CUtensorMap *vmap, PdShared<NT> &sm) {
         const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-        const uint64_t deadline = globaltimer_ns() + kPaTimeoutNs;
+        launch_dependents();
         if (lane == 0) {
             for (int i = 0; i < kPdStages; ++i) mbar_init(&sm.full[warp][i], 1);
             fence_mbar_init();
         }
+        grid_dependency_wait();
+        const uint64_t deadline = globaltimer_ns() + kPaTimeoutNs;
         // prefix sums of the sequences' units: each thread takes four consecutive sequences
         int mine[kSeqs], sum = 0;
 #pragma unroll
@@ -651,8 +653,7 @@ int pd_launch(const PaParams &p, const CUtensorMap &k, const CUtensorMap &v, cud
                                            (int)kPdSmem);
     });
     if (set_rc[dev] != cudaSuccess) return MMRS_ERR_LAUNCH;
-    paged_attend_decode_kernel<NT, T><<<pa_sm_count(), kPdThreads, kPdSmem, s>>>(p, k, v);
-    return cudaGetLastError() == cudaSuccess ? MMRS_OK : MMRS_ERR_LAUNCH;
+    return pg_launch(paged_attend_decode_kernel<NT, T>, (unsigned)pa_sm_count(), kPdThreads, kPdSmem, s, p, k, v);
 }
 
 template <typename T>
