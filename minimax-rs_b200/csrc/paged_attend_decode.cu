@@ -21,8 +21,8 @@
 // the workspace and the last to arrive joins them in order.
 //
 // Measured (48 + 8 heads): one token over 196608 positions 74 us (403 MB, 5.4 TB/s, 0.83 of a plain
-// copy's; the same ring without the arithmetic takes 67); one token over 4096 positions 11.2 us in a
-// captured graph (a chain of latencies: launch, lookups, first tiles, joins); 64 sequences of 1001 to 8192
+// copy's; the same ring without the arithmetic takes 67); one token over 4096 positions 11.6 us call
+// after call (a chain of latencies: launch, lookups, first tiles, joins); 64 sequences of 1001 to 8192
 // positions and 5 drafted tokens (30 rows) 250 us (612 MB, 2.5 TB/s): eight warps of 255 registers, each
 // with a chain of 128 products, 512 codes to turn and 32 exponentials a lane in a step, leave the
 // issue slots two thirds empty and memory at 0.37.  Twelve warps of 168 registers, two a step: 475 us.

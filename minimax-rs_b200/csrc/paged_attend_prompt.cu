@@ -36,7 +36,7 @@
 // cores are busy 40 % of the time and the exponential units 45 %: what is left is the chain of one
 // half, scores -> maximum -> exponentials -> P -> product, some 2500 cycles with two tiles to fill it
 // (half of the scores, three quarters of P V or all exponentials left out: 2 % less).  Five
-// ragged prompts of 1 to 2049 tokens with a window of 511, 32 + 4 heads: 167 us, of which 80 us are
+// ragged prompts of 1 to 2049 tokens with a window of 511, 32 + 4 heads: 165 us, of which 80 us are
 // full tiles' and most of the rest items' beginnings, ends and masked halves.
 #include "paged_attend.cuh"
 #include "umma.cuh"
