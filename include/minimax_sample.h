@@ -80,7 +80,8 @@ MMRS_API int mmrs_token_logprob(const float *logits, int vocab, int token_id, fl
 #define MMRS_VERIFY_MAX_Q 64
 
 /* Workspace bytes of mmrs_verify_drafts (0: arguments out of range).  Caller-owned, 256-byte
- * aligned, zero before first use; one workspace serves one stream at a time. */
+ * aligned, zero before first use; one workspace serves one stream at a time and calls of any size
+ * up to its own. */
 MMRS_API size_t mmrs_verify_workspace_bytes(int num_seqs, int total_rows);
 
 /* Outcome of the last completed call on a workspace (synchronous read): MMRS_OK, or

@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_choose_kernel(const VfPa
     float *logprobs = p.logprobs ? p.logprobs + (long)s * p.max_q : nullptr;
     const T *logits = static_cast<const T *>(p.logits);
     VfSeq *seq = p.seqs + s;
-    const int n = rows > 0 ? __ldcg(&seq->stood) : 0;
+    const int n = rows > 0 ? min(max(__ldcg(&seq->stood), 0), rows - 1) : 0;  // (a row of the sequence, whatever is there)
     const float top = __ldcg(&seq->top), sum = __ldcg(&seq->sum);
     const int row = row0 + n, at = row - s;
     const bool usable = rows > 0 && sum > 0.0f, fell = n < rows - 1 && at >= 0;
@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_choose_kernel(const VfPa
         if (threadIdx.x == 0) seq->count = 0;
     }
     if (threadIdx.x == 0) {
-        p.accepted[s] = max(n, 0);
+        p.accepted[s] = n;
         if (rows > 0 && next < 0) atomicExch(p.status, (uint32_t)MMRS_ERR_NONFINITE);
     }
     for (int i = warp; i < p.max_q; i += kVfWarps) {
@@ -378,19 +378,14 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_choose_kernel(const VfPa
     }
 }
 
-struct VfLayout {
-    size_t seqs, parts, total;
-};
-VfLayout vf_layout(int num_seqs, int total_rows) {
-    VfLayout l;
-    l.seqs = 256;
-    l.parts = l.seqs + (sizeof(VfSeq) * num_seqs + 255) / 256 * 256;
-    l.total = l.parts + sizeof(VfPart) * kVfChunks * (size_t)total_rows;
-    return l;
-}
+// Workspace: a status word, the sequences' records, the rows' parts.  The records' counters are zero from one
+// call to the next, so they lie where no call's size moves them (room for the most sequences, 287 KB): else a
+// call of few sequences would write its parts over the records that a larger one finds.
+constexpr size_t kVfSeqsAt = 256;
+constexpr size_t kVfPartsAt = kVfSeqsAt + (sizeof(VfSeq) * MMRS_VERIFY_MAX_SEQS + 255) / 256 * 256;
 size_t vf_workspace_bytes(int num_seqs, int total_rows) {
     if (num_seqs < 0 || num_seqs > MMRS_VERIFY_MAX_SEQS || total_rows < 0 || total_rows > MMRS_VERIFY_MAX_ROWS) return 0;
-    return vf_layout(num_seqs, total_rows).total;
+    return kVfPartsAt + sizeof(VfPart) * kVfChunks * (size_t)total_rows;
 }
 
 template <typename T>
@@ -467,10 +462,9 @@ extern "C" int mmrs_verify_drafts(const void *logits, int logits_type, int vocab
     p.chunks = (vocab + p.chunk - 1) / p.chunk;
     p.race_chunks = (vocab + p.race_chunk - 1) / p.race_chunk;
     uint8_t *ws = static_cast<uint8_t *>(workspace);
-    const VfLayout l = vf_layout(num_seqs, total_rows);
     p.status = reinterpret_cast<uint32_t *>(ws);
-    p.seqs = reinterpret_cast<VfSeq *>(ws + l.seqs);
-    p.parts = reinterpret_cast<VfPart *>(ws + l.parts);
+    p.seqs = reinterpret_cast<VfSeq *>(ws + kVfSeqsAt);
+    p.parts = reinterpret_cast<VfPart *>(ws + kVfPartsAt);
     cudaStream_t s = (cudaStream_t)stream;
     if (logits_type == MMRS_TYPE_F32) return vf_launch<float>(p, s);
     return logits_type == MMRS_TYPE_F16 ? vf_launch<__half>(p, s) : vf_launch<__nv_bfloat16>(p, s);
