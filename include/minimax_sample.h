@@ -92,7 +92,8 @@ MMRS_API int mmrs_verify_workspace_status(const void *workspace);
  * Sequence b has the logits rows cu_rows[b] .. cu_rows[b + 1] - 1 of logits [total_rows][vocab]
  * (logits_type MMRS_TYPE_F32, _F16 or _BF16 of minimax_paged.h): the target's rows after its last
  * accepted token and after each of its d = rows - 1 drafted tokens.  Draft i of it, element
- * cu_rows[b] - b + i of draft_tokens and uniforms and row of draft_probs [drafts][vocab] (the draft model's probabilities; null: the draft had probability 1), is judged by row i:
+ * cu_rows[b] - b + i of draft_tokens and uniforms and row of draft_probs [drafts][vocab] (the draft
+ * model's probabilities; null: the draft had probability 1), is judged by row i:
  *   temperature[b] == 0: it stands when it is the row's argmax (first index of the largest);
  *   otherwise, with p = softmax(logits / temperature[b]), when u * q(draft) < p(draft).
  * The drafts before the first that falls are emitted, then one more token: at temperature 0 the
@@ -112,6 +113,16 @@ MMRS_API int mmrs_verify_drafts(const void *logits, int logits_type, int vocab, 
                                 const float *uniforms, const float *noise, const float *temperature, int32_t *tokens,
                                 int32_t *accepted, float *logprobs, void *workspace, size_t workspace_bytes,
                                 mmrs_stream_t stream);
+
+/* The same with the number of drafts: draft_tokens and uniforms have num_drafts elements, draft_probs
+ * num_drafts rows, and nothing past them is read.  A draft that would lie there falls, and the next
+ * token is drawn from p of its row.  (mmrs_verify_drafts takes arrays that hold a draft for every
+ * row but each sequence's last; without them no draft stands.) */
+MMRS_API int mmrs_verify_drafts_n(const void *logits, int logits_type, int vocab, const int32_t *cu_rows, int num_seqs,
+                                  int total_rows, int max_q, const int32_t *draft_tokens, const float *draft_probs,
+                                  const float *uniforms, int num_drafts, const float *noise, const float *temperature,
+                                  int32_t *tokens, int32_t *accepted, float *logprobs, void *workspace,
+                                  size_t workspace_bytes, mmrs_stream_t stream);
 
 #ifdef __cplusplus
 }

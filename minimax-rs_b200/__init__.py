@@ -111,6 +111,7 @@ PROTOTYPES = {
     "mmrs_verify_workspace_bytes": (_SZ, [_I, _I]),
     "mmrs_verify_workspace_status": (_I, [_VP]),
     "mmrs_verify_drafts": (_I, [_VP, _I, _I, _VP, _I, _I, _I] + [_VP] * 9 + [_SZ, _VP]),
+    "mmrs_verify_drafts_n": (_I, [_VP, _I, _I, _VP, _I, _I, _I] + [_VP] * 3 + [_I] + [_VP] * 6 + [_SZ, _VP]),
     # paged 8-bit cache (include/minimax_paged.h)
     "mmrs_paged_append": (_I, [C.POINTER(MmrsPagedCache), C.POINTER(MmrsPagedBatch), _VP, _VP, _VP, _I64, _I64, _I64,
                                _I, _I, _VP, _VP, _I, _I, _VP, _I, _VP]),
@@ -665,7 +666,8 @@ class DraftVerifier:
         the drafts that stand and one more token a sequence, -1 (0.0) after them.  logits [rows][vocab]
         (f32, f16, bf16), cu_rows int32 [n + 1], draft_tokens int32 and uniforms f32 [drafts],
         draft_probs f32 [drafts][vocab] or None (drafts that were certain), noise f32 [n][vocab]
-        (exponential), temperature f32 [n] or None (1)."""
+        (exponential), temperature f32 [n] or None (1).  A row whose draft is not among them (sequences without
+        rows leave more rows to judge than rows - n) judges none: the next token is drawn there."""
         n, (rows, vocab) = cu_rows.numel() - 1, logits.shape
         drafts = draft_tokens.numel()
         if not 0 <= n <= self.max_seqs or rows > self.max_rows:
@@ -690,9 +692,9 @@ class DraftVerifier:
             if temperature.dtype != f32 or temperature.numel() != n or not temperature.is_contiguous():
                 raise MoeError(MMRS_ERR_ARG, "temperature f32 [n]")
             temp_ptr = temperature.data_ptr()
-        rc = lib().mmrs_verify_drafts(logits.data_ptr(), _type_code(logits.dtype), vocab, cu_rows.data_ptr(), n, rows,
-                                      self.max_q, draft_tokens.data_ptr(), probs_ptr, uniforms.data_ptr(),
-                                      noise.data_ptr(), temp_ptr, *self._ptrs, _raw_stream(stream, logits))
+        rc = lib().mmrs_verify_drafts_n(logits.data_ptr(), _type_code(logits.dtype), vocab, cu_rows.data_ptr(), n, rows,
+                                        self.max_q, draft_tokens.data_ptr(), probs_ptr, uniforms.data_ptr(), drafts,
+                                        noise.data_ptr(), temp_ptr, *self._ptrs, _raw_stream(stream, logits))
         if rc:
             raise MoeError(rc, "mmrs_verify_drafts")
         if n == self.max_seqs:

@@ -51,6 +51,7 @@ struct VfSeq {
 struct VfParams {
     const void *logits;
     int vocab, num_seqs, total_rows, max_q;
+    int num_drafts;               // elements of draft and u, rows of q
     int chunks, chunk;            // rows kernel: chunks of a row, tokens of a chunk
     int race_chunks, race_chunk;  // choose kernel
     const int32_t *cu, *draft;
@@ -162,7 +163,7 @@ __device__ __forceinline__ void vf_judge(const VfParams &p, int s, int row0, int
         const int row = row0 + r, at = row - s;
         float l = 0.0f, q = 1.0f, u = 0.0f;
         int tok = -1;
-        if (r < rows - 1 && at >= 0) {
+        if (r < rows - 1 && at >= 0 && at < p.num_drafts) {  // (no draft there: it falls)
             tok = p.draft[at], u = p.u[at];
             if (tok >= 0 && tok < p.vocab) {
                 l = pg_to_float(static_cast<const T *>(p.logits)[(long)row * p.vocab + tok]);
@@ -299,7 +300,7 @@ __global__ void __launch_bounds__(kVfThreads, 2) verify_choose_kernel(const VfPa
     const int n = rows > 0 ? min(max(__ldcg(&seq->stood), 0), rows - 1) : 0;  // (a row of the sequence, whatever is there)
     const float top = __ldcg(&seq->top), sum = __ldcg(&seq->sum);
     const int row = row0 + n, at = row - s;
-    const bool usable = rows > 0 && sum > 0.0f, fell = n < rows - 1 && at >= 0;
+    const bool usable = rows > 0 && sum > 0.0f, fell = n < rows - 1 && at >= 0 && at < p.num_drafts;
     const T *l = logits + (long)row * p.vocab;
     const float *q = fell && p.q ? p.q + (long)at * p.vocab : nullptr;
     const int gone = fell && !p.q ? p.draft[at] : -1;
@@ -421,25 +422,25 @@ extern "C" int mmrs_verify_workspace_status(const void *workspace) {
     return (int)st;
 }
 
-extern "C" int mmrs_verify_drafts(const void *logits, int logits_type, int vocab, const int32_t *cu_rows, int num_seqs,
-                                  int total_rows, int max_q, const int32_t *draft_tokens, const float *draft_probs,
-                                  const float *uniforms, const float *noise, const float *temperature, int32_t *tokens,
-                                  int32_t *accepted, float *logprobs, void *workspace, size_t workspace_bytes,
-                                  mmrs_stream_t stream) {
+extern "C" int mmrs_verify_drafts_n(const void *logits, int logits_type, int vocab, const int32_t *cu_rows, int num_seqs,
+                                    int total_rows, int max_q, const int32_t *draft_tokens, const float *draft_probs,
+                                    const float *uniforms, int num_drafts, const float *noise, const float *temperature,
+                                    int32_t *tokens, int32_t *accepted, float *logprobs, void *workspace,
+                                    size_t workspace_bytes, mmrs_stream_t stream) {
     if (logits_type < MMRS_TYPE_F32 || logits_type > MMRS_TYPE_BF16) return MMRS_ERR_UNSUPPORTED;
     if (vocab < 1 || vocab > MMRS_SAMPLE_MAX_VOCAB || num_seqs < 0 || num_seqs > MMRS_VERIFY_MAX_SEQS ||
-        total_rows < 0 || total_rows > MMRS_VERIFY_MAX_ROWS || max_q < 1 || max_q > MMRS_VERIFY_MAX_Q)
+        total_rows < 0 || total_rows > MMRS_VERIFY_MAX_ROWS || max_q < 1 || max_q > MMRS_VERIFY_MAX_Q || num_drafts < 0)
         return MMRS_ERR_ARG;
     if (num_seqs == 0) return MMRS_OK;
     if (!cu_rows || !tokens || !accepted) return MMRS_ERR_ARG;
     if (total_rows && (!logits || !noise)) return MMRS_ERR_ARG;
-    // a sequence may have no rows, so only more rows than sequences are known to bring drafts
-    if (total_rows > num_seqs && (!draft_tokens || !uniforms)) return MMRS_ERR_ARG;
+    if (num_drafts && (!draft_tokens || !uniforms)) return MMRS_ERR_ARG;
     if (!workspace || ((uintptr_t)workspace & 255u) || workspace_bytes < vf_workspace_bytes(num_seqs, total_rows))
         return MMRS_ERR_ARG;
     VfParams p = {};
     p.logits = logits;
     p.vocab = vocab, p.num_seqs = num_seqs, p.total_rows = total_rows, p.max_q = max_q;
+    p.num_drafts = num_drafts;
     p.cu = cu_rows, p.draft = draft_tokens;
     p.q = draft_probs, p.u = uniforms, p.noise = noise, p.temperature = temperature;
     p.tokens = tokens, p.accepted = accepted, p.logprobs = logprobs;
@@ -468,4 +469,18 @@ extern "C" int mmrs_verify_drafts(const void *logits, int logits_type, int vocab
     cudaStream_t s = (cudaStream_t)stream;
     if (logits_type == MMRS_TYPE_F32) return vf_launch<float>(p, s);
     return logits_type == MMRS_TYPE_F16 ? vf_launch<__half>(p, s) : vf_launch<__nv_bfloat16>(p, s);
+}
+
+extern "C" int mmrs_verify_drafts(const void *logits, int logits_type, int vocab, const int32_t *cu_rows, int num_seqs,
+                                  int total_rows, int max_q, const int32_t *draft_tokens, const float *draft_probs,
+                                  const float *uniforms, const float *noise, const float *temperature, int32_t *tokens,
+                                  int32_t *accepted, float *logprobs, void *workspace, size_t workspace_bytes,
+                                  mmrs_stream_t stream) {
+    // How many sequences have rows is on the device: more rows than sequences bring drafts for certain; without
+    // the arrays there are none, with them as many as the rows ask for.
+    const bool given = draft_tokens && uniforms;
+    if (total_rows > num_seqs && num_seqs > 0 && !given) return MMRS_ERR_ARG;
+    return mmrs_verify_drafts_n(logits, logits_type, vocab, cu_rows, num_seqs, total_rows, max_q, draft_tokens, draft_probs,
+                                uniforms, given && total_rows > 0 ? total_rows : 0, noise, temperature, tokens, accepted,
+                                logprobs, workspace, workspace_bytes, stream);
 }
