@@ -730,11 +730,12 @@ __device__ void pp_softmax(const PaParams &p, PpShared &sm, int u0, int u1, int 
             }
         }
         // The next piece's queries, so that its first scores are under way while this one's O is read: the
-        // scores that used these queries have all been here.
+        // scores that used these queries have all been here.  (After a failed wait the walk goes on, too: all
+        // warps reach the barriers of the same cut items.)
         PpSeg next = s;
-        if (ok && u + s.n < u1) {
+        if (u + s.n < u1) {
             pp_next(p, sm, u + s.n, u1, lane, next);
-            queries(next);
+            if (ok) queries(next);
         }
         if (ok && mine) {
             ok = pp_wait_warp(&sm.o_done[i][1], (uint32_t)(used + s.n - 1) & 1, sm, p);
