@@ -82,7 +82,8 @@ MMRS_API int mmrs_paged_append(const MmrsPagedCache *cache, const MmrsPagedBatch
 MMRS_API size_t mmrs_paged_attend_workspace_bytes(int num_seqs, int total_q, int query_heads, int kv_heads);
 
 /* Outcome of the completed calls on a workspace (synchronous read): MMRS_OK, or MMRS_ERR_TIMEOUT
- * when a bounded wait inside a kernel expired (outputs are then incomplete). */
+ * when a bounded wait inside a kernel expired: the outputs of that call are incomplete.  The workspace
+ * stays usable; its status word keeps the error until the caller zeroes it. */
 MMRS_API int mmrs_paged_attend_status(const void *workspace);
 
 /* Attention of the batch's token rows over the cache.  q [total_q][query_heads][128] of `type` (f16

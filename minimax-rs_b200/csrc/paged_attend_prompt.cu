@@ -775,7 +775,9 @@ __device__ void pp_softmax(const PaParams &p, PpShared &sm, int u0, int u1, int 
             named_sync(1, 256);
             if (threadIdx.x == 0) {
                 __threadfence();
-                sm.last = !sm.abort && atomicAdd(p.counters + c0, 1u) == (uint32_t)(c1 - c0);
+                // (a block that gave up counts, too: the last one puts the counter back to zero, and the status says
+                // that the rows are incomplete)
+                sm.last = atomicAdd(p.counters + c0, 1u) == (uint32_t)(c1 - c0);
                 __threadfence();
             }
             named_sync(1, 256);

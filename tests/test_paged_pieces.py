@@ -69,3 +69,29 @@ def test_the_model_tells_the_rules_apart():
 
 def test_every_warp_reaches_the_same_barriers_after_a_failed_wait():
     assert disagreements(advances_when_failed()) == 0
+
+
+def counts_when_failed() -> bool:
+    """Whether a block that gave up counts as arrived at the cut items it held a piece of."""
+    rule = re.search(r"sm\.last = ([^;]*)atomicAdd\(p\.counters \+ c0, 1u\)", SOURCE.read_text())
+    assert rule, "the block's arrival at a cut item"
+    return "abort" not in rule.group(1)
+
+
+def test_every_call_leaves_the_counters_at_zero():
+    """An item's last block to arrive puts its counter back: so every block has to arrive, one that gave up, too.
+    (The next call on the workspace would otherwise take an earlier block for the last and join too soon.)"""
+    r, every = random.Random(6), counts_when_failed()
+    for _ in range(200):
+        items = [r.randint(1, 12) for _ in range(r.randint(1, 30))]
+        share = max(1, -(-sum(items) // r.randint(1, 12)))
+        blocks = -(-sum(items) // share)
+        counters, failed = [0] * blocks, [r.random() < 0.3 for _ in range(blocks)]
+        for block in r.sample(range(blocks), blocks):
+            todo, u, _ = pieces(items, share, block)
+            for item, off, n in todo:
+                c0, c1 = (u - off) // share, (u - off + items[item] - 1) // share
+                if c0 != c1 and (every or not failed[block]):
+                    counters[c0] = 0 if counters[c0] == c1 - c0 else counters[c0] + 1
+                u += n
+        assert not any(counters)
