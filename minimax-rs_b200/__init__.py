@@ -555,6 +555,7 @@ class PagedKvCache:
                                 self.page_size, self.kv_heads)
         self._ref = C.byref(self.c)
         self.ws, self._ws_need = None, {}  # workspace bytes by (sequences, tokens, query heads)
+        self._spaces = []  # every workspace handed out: captured graphs go on using the one that they were captured with
 
     def append(self, batch: PagedBatch, q, k, v, rope_cos, rope_sin, q_out=None, stream=None):
         """Writes the rotated k and v [tokens][kv_heads][128] (f32, f16 or bf16; row slices of one wider
@@ -594,7 +595,10 @@ class PagedKvCache:
         return q_out
 
     def workspace(self, num_seqs: int, tokens: int, query_heads: int, stream=None):
-        """The attention's workspace, large enough for such a call; a new one is zeroed on `stream`."""
+        """The attention's workspace, large enough for such a call; a new one is zeroed on `stream`.  There are two
+        sizes (up to 48 rows a KV head, 5 MB, and above, 39 MB); a smaller one stays as long as the cache, for the
+        graphs that were captured with it.  None is made inside a capture, where the zeroing would only be
+        recorded: call this, or `attend`, for the largest call before it."""
         key = (num_seqs, tokens, query_heads)
         need = self._ws_need.get(key)
         if need is None:
@@ -605,20 +609,24 @@ class PagedKvCache:
         if self.ws is None or self.ws.numel() < need:
             import torch
             with _on_stream(stream):
+                if self.device_index >= 0 and torch.cuda.is_current_stream_capturing():
+                    raise MoeError(MMRS_ERR_ARG, "a workspace cannot be made inside a capture: call workspace() before it")
                 self.ws = torch.zeros(need, dtype=torch.uint8, device=self.k.device)
+            self._spaces.append(self.ws)
             self._ws_ptr, self._ws_bytes = self.ws.data_ptr(), need
         return self.ws
 
     def status(self) -> int:
         """MMRS_OK, or MMRS_ERR_TIMEOUT when a bounded wait in an attention kernel expired (synchronous)."""
-        return MMRS_OK if self.ws is None else lib().mmrs_paged_attend_status(self.ws.data_ptr())
+        return next((st for st in (lib().mmrs_paged_attend_status(w.data_ptr()) for w in self._spaces) if st), MMRS_OK)
 
     def attend(self, batch: PagedBatch, q, scale: float | None = None, window: int = 0, sinks: int = 0, out=None,
                lse=None, stream=None):
         """out [tokens][heads][128] = attention of q (f16 or bf16, rotated) over the batch's positions up to
         each token's own; with window > 0 only the last `window` of them and the first `sinks`.  lse
         f32 [tokens][heads] is filled when given.  scale: 1 / sqrt(128) unless given.  The calls of
-        one cache share a workspace: keep them on one stream."""
+        one cache share a workspace: keep them on one stream.  A captured call needs the cache (which owns the
+        workspace) for as long as its graph is replayed, and a call of its size, or `workspace`, before it."""
         n, heads, stride = _tokens(q, None, "q")
         _same_device(self.device_index, batch.t[1], q, out, lse)
         if out is None:
