@@ -447,14 +447,6 @@ def _need(ok: bool, what: str) -> None:
         raise MoeError(MMRS_ERR_ARG, what)
 
 
-def _raw_stream(stream, t) -> int:
-    """The handle of `stream`, or of the current stream of t's device (without making a Stream object)."""
-    if stream is not None:
-        return stream.cuda_stream
-    import torch
-    return torch._C._cuda_getCurrentRawStream(t.get_device())
-
-
 def _on_stream(stream):
     """Where a call allocates: on the stream it runs on, which then owns the memory."""
     import contextlib
@@ -484,6 +476,13 @@ def _tokens(t, heads, what: str):
     if d != HEAD_DIM or one != 1 or h != (heads or h) or h < 1 or (head != HEAD_DIM and h > 1):
         raise MoeError(MMRS_ERR_ARG, f"{what}: [tokens][{heads or 'heads'}][{HEAD_DIM}], heads side by side")
     return n, h, row if n > 1 else max(row, h * HEAD_DIM)
+
+
+def _on_gpu(dev: int):
+    """Makes GPU `dev` the current one.  A kernel is launched on the current GPU whatever its pointers: a call
+    for tensors of another one runs inside this."""
+    import torch
+    return torch.cuda.device(dev)
 
 
 class PagedBatch:
@@ -554,6 +553,8 @@ class PagedKvCache:
         self.c = MmrsPagedCache(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages,
                                 self.page_size, self.kv_heads)
         self._ref = C.byref(self.c)
+        # the GPU that launches go to; the handle of a GPU's current stream (without making a Stream object)
+        self._gpu_now, self._raw_now = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
         self.ws, self._ws_need = None, {}  # workspace bytes by (sequences, tokens, query heads)
         self._spaces = []  # every workspace handed out: captured graphs go on using the one that they were captured with
 
@@ -564,6 +565,9 @@ class PagedKvCache:
         dtype = k.dtype
         code = _type_code(dtype)
         _same_device(self.device_index, batch.t[1], q, k, v, rope_cos, rope_sin, q_out)
+        if self._gpu_now() != self.device_index:
+            with _on_gpu(self.device_index):
+                return self.append(batch, q, k, v, rope_cos, rope_sin, q_out, stream)
         n, _, k_stride = _tokens(k, self.kv_heads, "k")
         v_n, _, v_stride = _tokens(v, self.kv_heads, "v")
         if v_n != n or v.dtype is not dtype:
@@ -589,7 +593,8 @@ class PagedKvCache:
             q_ptr, out_ptr = q.data_ptr(), q_out.data_ptr()
         rc = lib().mmrs_paged_append(self._ref, batch.bind(self, n), q_ptr, k.data_ptr(), v.data_ptr(), q_stride,
                                      k_stride, v_stride, code, heads, rope_cos.data_ptr(), rope_sin.data_ptr(),
-                                     2 * rope[1], rope[0], out_ptr, out_code, _raw_stream(stream, k))
+                                     2 * rope[1], rope[0], out_ptr, out_code,
+                                     self._raw_now(self.device_index) if stream is None else stream.cuda_stream)
         if rc:
             raise MoeError(rc, "mmrs_paged_append")
         return q_out
@@ -629,6 +634,9 @@ class PagedKvCache:
         workspace) for as long as its graph is replayed, and a call of its size, or `workspace`, before it."""
         n, heads, stride = _tokens(q, None, "q")
         _same_device(self.device_index, batch.t[1], q, out, lse)
+        if self._gpu_now() != self.device_index:
+            with _on_gpu(self.device_index):
+                return self.attend(batch, q, scale, window, sinks, out, lse, stream)
         if out is None:
             import torch
             with _on_stream(stream):
@@ -643,7 +651,8 @@ class PagedKvCache:
         self.workspace(batch.num_seqs, n, heads, stream)
         rc = lib().mmrs_paged_attend(self._ref, batch.bind(self, n), q.data_ptr(), stride, _type_code(q.dtype), heads,
                                      HEAD_DIM ** -0.5 if scale is None else scale, window, sinks, out.data_ptr(), lse_ptr,
-                                     self._ws_ptr, self._ws_bytes, _raw_stream(stream, q))
+                                     self._ws_ptr, self._ws_bytes,
+                                     self._raw_now(self.device_index) if stream is None else stream.cuda_stream)
         if rc:
             raise MoeError(rc, "mmrs_paged_attend")
         return out
@@ -659,6 +668,8 @@ class DraftVerifier:
         if need == 0 or max_seqs < 1:
             raise MoeError(MMRS_ERR_ARG, "mmrs_verify_workspace_bytes")
         self.vocab, self.max_seqs, self.max_rows, self.max_q = vocab, max_seqs, max_rows, max_q
+        # the GPU that launches go to; the handle of a GPU's current stream (without making a Stream object)
+        self._gpu_now, self._raw_now = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
         self.ws = torch.zeros(need, dtype=torch.uint8, device=device)
         self.tokens = torch.full((max_seqs, max_q), -1, dtype=torch.int32, device=device)
         self.accepted = torch.zeros(max_seqs, dtype=torch.int32, device=device)
@@ -682,7 +693,11 @@ class DraftVerifier:
             raise MoeError(MMRS_ERR_ARG, "more sequences or rows than the verifier was made for")
         if vocab != self.vocab or not logits.is_contiguous():
             raise MoeError(MMRS_ERR_ARG, "logits [rows][vocab]")
-        _same_device(self.tokens.get_device(), logits, cu_rows, draft_tokens, uniforms, noise, draft_probs, temperature)
+        dev = self.tokens.get_device()
+        _same_device(dev, logits, cu_rows, draft_tokens, uniforms, noise, draft_probs, temperature)
+        if self._gpu_now() != dev:
+            with _on_gpu(dev):
+                return self.verify(logits, cu_rows, draft_tokens, uniforms, noise, draft_probs, temperature, stream)
         i32, f32 = self.tokens.dtype, self.logprobs.dtype
         if (cu_rows.dtype != i32 or draft_tokens.dtype != i32 or not cu_rows.is_contiguous() or
                 not draft_tokens.is_contiguous()):
@@ -702,7 +717,8 @@ class DraftVerifier:
             temp_ptr = temperature.data_ptr()
         rc = lib().mmrs_verify_drafts_n(logits.data_ptr(), _type_code(logits.dtype), vocab, cu_rows.data_ptr(), n, rows,
                                         self.max_q, draft_tokens.data_ptr(), probs_ptr, uniforms.data_ptr(), drafts,
-                                        noise.data_ptr(), temp_ptr, *self._ptrs, _raw_stream(stream, logits))
+                                        noise.data_ptr(), temp_ptr, *self._ptrs,
+                                        self._raw_now(dev) if stream is None else stream.cuda_stream)
         if rc:
             raise MoeError(rc, "mmrs_verify_drafts")
         if n == self.max_seqs:
