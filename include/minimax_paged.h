@@ -92,9 +92,12 @@ MMRS_API int mmrs_paged_attend_status(const void *workspace);
  * with window > 0, of those only p - j < window and j < sinks (the first tokens stay visible).
  * out [total_q][query_heads][128] of `type` = softmax(scale q k) v; lse f32 [total_q][query_heads]
  * (or null) = ln sum exp(scale q k).  A row that sees nothing gives 0 and -infinity.  Statistics
- * and sums are f32; probabilities are rounded to f16 for the second product, bf16 queries go to f16
- * after an exact power-of-two scaling of their row, and value scales relative to the largest one met
- * are rounded to f16 (exact for the powers of two that the append writes). */
+ * and sums are f32; probabilities are rounded to f16 for the second product, and bf16 queries go to f16
+ * after a power-of-two scaling of their row (exact down to 2^-31 of its largest value).
+ *   Value scales enter that product relative to a reference scale, rounded to f16 (exact for the powers
+ * of two that the append writes).  For a sequence of up to 48 rows a KV head the reference follows the
+ * pages, to within 2^6: pages may lie 2^64 apart.  For longer ones the values take the ratio to the
+ * largest scale met: they keep their bits down to 2^-15 of it and are zero below 2^-34. */
 MMRS_API int mmrs_paged_attend(const MmrsPagedCache *cache, const MmrsPagedBatch *batch, const void *q,
                                int64_t q_stride, int type, int query_heads, float scale, int window, int sinks,
                                void *out, float *lse, void *workspace, size_t workspace_bytes, mmrs_stream_t stream);

@@ -14,6 +14,11 @@
 // fits f16), found by one vote over the step's scores: the usual step neither reduces a maximum over
 // lanes nor touches O.
 //
+// Value scales: P takes the ratio of its page's scale to the warp's reference, a power of two in f16.  The
+// reference moves, and O with it, only for a page that has weight and lies above twice or below 1/64 of it.
+// (A reference that went up only lost every value on pages 2^24 and more below the largest one met, and
+// bits from 2^-14 on; the time is the same, 242 instead of 250 us for the drafts below.)
+//
 // Work: the steps of 32 positions of all sequences and KV heads form one list, of which every CTA
 // (one per SM) takes an equal, contiguous part; a CTA's warps take its steps in turn, each
 // with a ring of TMA copies of its own, its own running maximum and sum, and no barrier until the end
@@ -23,7 +28,7 @@
 // Measured (48 + 8 heads): one token over 196608 positions 74 us (403 MB, 5.4 TB/s, 0.83 of a plain
 // copy's; the same ring without the arithmetic takes 67); one token over 4096 positions 11.6 us call
 // after call (a chain of latencies: launch, lookups, first tiles, joins); 64 sequences of 1001 to 8192
-// positions and 5 drafted tokens (30 rows) 250 us (612 MB, 2.5 TB/s): eight warps of 255 registers, each
+// positions and 5 drafted tokens (30 rows) 242 us (612 MB, 2.5 TB/s): eight warps of 255 registers, each
 // with a chain of 128 products, 512 codes to turn and 32 exponentials a lane in a step, leave the
 // issue slots two thirds empty and memory at 0.37.  Twelve warps of 168 registers, two a step: 475 us.
 #include "paged_attend.cuh"
@@ -38,6 +43,7 @@ constexpr int kPdStep = 32;                       // positions of a step: two gr
 constexpr int kPdTile = kPdStep * kPgDim;         // bytes of its keys (or values)
 constexpr float kPdLazy = 8.0f;                   // log2 of how far P may exceed 1
 constexpr float kPdNone = -1e30f;                 // below every score
+constexpr float kPdUnder = 1.0f / 64;             // how far a page's value scale may lie below the warp's reference
 constexpr int kPdRowFloats = kPgDim + 4;          // a row of the merge buffer
 
 constexpr int kPdWarps = 8;
@@ -331,16 +337,40 @@ struct PdKernel {
                 }
             const int pos_lo = s.seq.pos0, pos_hi = s.seq.len - 1;
             float m[NT][2], l[NT][2], o[NT][8][4];  // per column; the maximum kPdNone before the first score
-            float vref = 0.0f;
+            float vref = 0.0f, vinv = 0.0f;  // the values' reference scale, 0 before the first
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                for (int c = 0; c < 2; ++c) m[nt][c] = kPdNone, l[nt][c] = 0.0f;
+                for (int c = 0; c < 2; ++c) m[nt][c] = pos[nt][c] < 0 ? -kPdNone : kPdNone, l[nt][c] = 0.0f;  // (no row: P = 0)
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
 #pragma unroll
                     for (int c = 0; c < 4; ++c) o[nt][j][c] = 0.0f;
             }
+            // The sums O to another reference.  Downwards they grow: by no more than takes the largest of them to
+            // 2^100, for a page so far below it that f32 could not hold both.
+            auto move = [&](float to) {
+                float f = vref / to;
+                if (f > 1.0f) {
+                    float most = 0x1p-20f;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) most = fmaxf(most, fabsf(o[nt][j][c]));
+                    most = fminf(warp_max_butterfly(most), 0x1p100f);  // (an infinity stays one)
+                    f = fminf(f, 0x1p100f / __uint_as_float(__float_as_uint(most) & 0x7f800000u));
+                    to = vref / f;
+                }
+                vref = to, vinv = 1.0f / to;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) o[nt][j][c] *= f;
+            };
             for (int i = warp; i < s.n; i += kPdWarps, ++used) {
                 const int st = used % kPdStages;
                 if (!failed && !mbar_wait_bounded(&sm.full[warp][st], (used / kPdStages) & 1, deadline)) {
@@ -414,11 +444,11 @@ struct PdKernel {
 #pragma unroll
                         for (int c = 0; c < 2; ++c)
                             over = over || largest(nt, c) > m[nt][c] + kPdLazy;
-                    // the values' scale: probabilities are stored relative to the largest seen
-                    const float vtop = kE == 2 ? fmaxf(vsc[0], vsc[1]) : vsc[e0];
-                    if (vtop > vref || __any_sync(0xffffffffu, over)) {
-                        const float vfac = vtop > vref ? vref / vtop : 1.0f;
-                        vref = fmaxf(vref, vtop);
+                    if (__any_sync(0xffffffffu, over)) {
+                        if (vref == 0.0f) {  // the first page's scale, here (O is zero) rather than by a branch of its own
+                            vref = kE == 2 ? fmaxf(vsc[0], vsc[1]) : vsc[e0];
+                            vinv = vref > 0.0f ? 1.0f / vref : 0.0f;
+                        }
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -428,18 +458,16 @@ struct PdKernel {
                                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
                                 mx = fmaxf(mx, m[nt][c]);
-                                const float fac = pa_exp2(m[nt][c] - mx), of = fac * vfac;
+                                const float fac = pa_exp2(m[nt][c] - mx);
                                 m[nt][c] = mx;
                                 l[nt][c] *= fac;
 #pragma unroll
-                                for (int j = 0; j < 8; ++j) o[nt][j][c] *= of, o[nt][j][c + 2] *= of;
+                                for (int j = 0; j < 8; ++j) o[nt][j][c] *= fac, o[nt][j][c + 2] *= fac;
                             }
                     }
-                    const float vinv = vref > 0.0f ? 1.0f / vref : 0.0f;
                     uint32_t pb[kE][NT][2];
 #pragma unroll
                     for (int e = 0; e < kE; ++e) {
-                        const __half2 vr = __float2half2_rn(vsc[e0 + e] * vinv);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
                             float p4[4];
@@ -450,17 +478,35 @@ struct PdKernel {
                                 p4[c + 2] = pa_exp2(fmaf(sc[e][nt][c + 2], f, -m[nt][c]));
                                 l[nt][c] += p4[c] + p4[c + 2];
                             }
-                            // (a product of halves: exact for scales that are powers of two)
-                            auto pack = [&](float x, float y) {
-                                const __half2 z = __hmul2(__floats2half2_rn(x, y), vr);
-                                return pd_transpose(*reinterpret_cast<const uint32_t *>(&z));
-                            };
-                            pb[e][nt][0] = pack(p4[0], p4[1]);
-                            pb[e][nt][1] = pack(p4[2], p4[3]);
+                            pb[e][nt][0] = pd_transpose(pg_pack2(p4[0], p4[1], (const __half *)nullptr));
+                            pb[e][nt][1] = pd_transpose(pg_pack2(p4[2], p4[3], (const __half *)nullptr));
                         }
                     }
 #pragma unroll
                     for (int e = 0; e < kE; ++e) {
+                        // The values' scale enters P relative to the warp's reference, which follows the pages up, and
+                        // down where one lies far below it (P times the ratio keeps f16's eleven bits down to 2^-8); a
+                        // page without any weight, or whose values are all zero, does not move it.
+                        float ratio = vsc[e0 + e] * vinv;
+                        if (__float_as_uint(ratio) - __float_as_uint(kPdUnder) >= __float_as_uint(2.0f) - __float_as_uint(kPdUnder)) {
+                            uint32_t some = 0;
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) some |= pb[e][nt][0] | pb[e][nt][1];
+                            ratio = 0.0f;
+                            if (vsc[e0 + e] > 0.0f && __any_sync(0xffffffffu, some != 0)) {
+                                move(vsc[e0 + e]);
+                                ratio = vsc[e0 + e] * vinv;
+                            }
+                        }
+                        // (a product of halves: exact for scales that are powers of two)
+                        const __half2 vr = __float2half2_rn(ratio);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int c = 0; c < 2; ++c) {
+                                const __half2 z = __hmul2(*reinterpret_cast<const __half2 *>(&pb[e][nt][c]), vr);
+                                pb[e][nt][c] = *reinterpret_cast<const uint32_t *>(&z);
+                            }
                         uint4 v4[4];
 #pragma unroll
                         for (int c = 0; c < 4; ++c) {

@@ -23,6 +23,7 @@ import torch
 from paged_cases import D, Case, code_values
 
 RATIO = 2.0 ** 6
+FEW_ROWS = 48  # of a KV head: up to these a sequence counts as single tokens or drafts
 FACTOR = 4.0
 
 
@@ -39,6 +40,7 @@ def attend_fine(c: Case, q: torch.Tensor, scale=D ** -0.5, window=0, sinks=0, dr
         if n_new == 0 or n <= 0:
             continue
         rows = slice(int(c.cu[b]), int(c.cu[b + 1]))
+        prompt = n_new * group > FEW_ROWS
         at = c.table[b, :-(-n // c.page)].long()
         inside = ((at >= 0) & (at < c.pages)).repeat_interleave(c.page)[:n]
         at = at.clamp(0, c.pages - 1)
@@ -52,7 +54,7 @@ def attend_fine(c: Case, q: torch.Tensor, scale=D ** -0.5, window=0, sinks=0, dr
             v = code_values(c.v[at, kv]).flatten(0, 1)[:n] * vs[:, None]
             v = torch.where(inside[:, None], v, torch.zeros_like(v))
             vs = torch.where(inside, vs, torch.zeros_like(vs))
-            ratio = (vs.max() / vs.clamp_min(1e-300)).clamp_max(RATIO)
+            ratio = (vs.max() / vs.clamp_min(1e-300)).clamp_max(0.0 if prompt else RATIO)
             tile = torch.stack([x.max() for x in vs.split(128)]).repeat_interleave(128)[:n]
             kept = v.clone()
             if drop_page is not None and drop_page[0] == b:
@@ -73,7 +75,7 @@ def attend_fine(c: Case, q: torch.Tensor, scale=D ** -0.5, window=0, sinks=0, dr
                 square = each ** 2 @ v ** 2 + (unit * out[rows, h]) ** 2 / 3 + 2.0 ** -50
                 walk = (w ** 2 @ v ** 2).mean(1).sqrt() + out[rows, h].square().mean(1).sqrt()
                 rms[rows, h] = FACTOR * square.mean(1).sqrt() + sums * walk
-                low = torch.minimum(v.abs(), (2.0 ** -24 * tile)[:, None]) * (vs < 2.0 ** -22 * tile)[:, None]
+                low = torch.minimum(v.abs(), (2.0 ** -24 * tile)[:, None]) * (prompt & (vs < 2.0 ** -22 * tile))[:, None]
                 allow[rows, h] = err @ v.abs() + w @ low
                 rms[rows, h] += (w @ low).square().mean(1).sqrt()
                 lse[rows, h] = (m + z.log())[:, 0]
