@@ -95,9 +95,10 @@ MMRS_API int mmrs_paged_attend_status(const void *workspace);
  * and sums are f32; probabilities are rounded to f16 for the second product, and bf16 queries go to f16
  * after a power-of-two scaling of their row (exact down to 2^-31 of its largest value).
  *   Value scales enter that product relative to a reference scale, rounded to f16 (exact for the powers
- * of two that the append writes).  For a sequence of up to 48 rows a KV head the reference follows the
- * pages, to within 2^6: pages may lie 2^64 apart.  For longer ones the values take the ratio to the
- * largest scale met: they keep their bits down to 2^-15 of it and are zero below 2^-34. */
+ * of two that the append writes), which follows the pages.  For a sequence of up to 48 rows a KV head
+ * pages may lie 2^64 apart without values being lost next to larger ones.  For longer ones that holds
+ * between runs of 128 positions (from a multiple of 128 on) up to 2^60; within one, values keep their
+ * bits down to 2^-22 of its largest scale and lose them one by one below. */
 MMRS_API int mmrs_paged_attend(const MmrsPagedCache *cache, const MmrsPagedBatch *batch, const void *q,
                                int64_t q_stride, int type, int query_heads, float scale, int window, int sinks,
                                void *out, float *lse, void *workspace, size_t workspace_bytes, mmrs_stream_t stream);

@@ -18,10 +18,12 @@
 // product's N, so the tile is read MN-major).
 //
 // Scales: a page's key scale multiplies its columns' scores in the exponent's FMA.  Its value scale,
-// relative to the largest of the piece, multiplies the values on their way to f16 (exact for the
-// powers of two that the append writes, one rounding otherwise).  Neither costs the softmax anything
-// an element.  The running maximum moves only when it grows by more than 2^8 (P stays below f16's
-// range), which leaves O alone on almost every tile.
+// relative to a reference, multiplies the values on their way to f16 (exact for the powers of two that the
+// append writes, one rounding otherwise).  Neither costs the softmax anything an element.  The reference is the
+// piece's, from its largest scale; where scales lie more than 2^22 apart, it is each tile's, and O is rescaled
+// with it as with the maximum.  (One reference for the piece and nothing else took 1427 us instead of 1451 at the
+// prompt below, and lost the values of pages 2^26 below the largest.)  The running maximum moves only when it
+// grows by more than 2^8 (P stays below f16's range), which leaves O alone on almost every tile.
 //
 // Masks: a half that all of a warp's rows see whole costs one vote; one that none sees is left out; else
 // 64 visibility bits a row choose between scores in registers (a pass through tensor memory of their
@@ -31,12 +33,12 @@
 // per SM) takes an equal contiguous part; an item cut by that gets its pieces joined through the
 // workspace by the CTA that finishes last, in order.
 //
-// Measured: 4096 tokens behind 12288 others, 48 + 8 heads, f16: 1430 us from a cold start (1010 TFLOP/s,
-// 0.62 of what the library's largest product reaches), some 1600 us under the power limit.  The tensor
+// Measured: 4096 tokens behind 12288 others, 48 + 8 heads, f16: 1451 us from a cold start (994 TFLOP/s,
+// 0.61 of what the library's largest product reaches), some 1690 us under the power limit.  The tensor
 // cores are busy 40 % of the time and the exponential units 45 %: what is left is the chain of one
 // half, scores -> maximum -> exponentials -> P -> product, some 2500 cycles with two tiles to fill it
 // (half of the scores, three quarters of P V or all exponentials left out: 2 % less).  Five
-// ragged prompts of 1 to 2049 tokens with a window of 511, 32 + 4 heads: 165 us, of which 80 us are
+// ragged prompts of 1 to 2049 tokens with a window of 511, 32 + 4 heads: 160 us, of which 80 us are
 // full tiles' and most of the rest items' beginnings, ends and masked halves.
 #include "paged_attend.cuh"
 #include "umma.cuh"
@@ -54,17 +56,23 @@ constexpr int kPpSlice = 128 * 16;           // bytes between 8-column slices of
 constexpr int kPpStages = 2;
 constexpr int kPpScales = 4;                 // tiles whose scales are kept
 constexpr float kPpLazy = 8.0f;              // log2 of how far P may exceed 1
+// The largest value scale in units of the reference: codes (up to 448) times it stay in f16's range.  A code times
+// the least scale that kPpExact allows for keeps its bits (e4m3's subnormals end at 2^-9, f16's at 2^-24).
+constexpr float kPpAbove = 128.0f;
+constexpr float kPpExact = 0x1p-22f;  // least over largest
+constexpr float kPpDown = 0x1p-60f;   // how far below the largest one met the reference follows (O stays below 2^104)
 constexpr int kPpConvWarp0 = 8, kPpMmaWarp = 12;
 
 struct alignas(16) PpScale {  // of the eight 16-position groups of a tile
     float k[8];  // key scale; < 0: the group's page holds nothing
-    float vref;  // what the piece's values are relative to
+    float vref;  // what the tile's values are relative to
 };
 struct PpShared {
     uint8_t q[2][kPpTile], k[kPpStages][kPpTile], v[kPpStages][kPpTile];
     float row_top[kPpRows], row_inv[kPpRows];  // of an item's rows while its pieces are joined
     PpScale sc[kPpScales];
-    float vmax[4];
+    float2 vrange[4];  // largest and least value scale of a converter warp's groups
+    float high[4], unit[4];  // a converter warp's reference, and pp_follow's largest scale (negative: one reference a piece)
     int prefix[kPaMaxSeqs + 1];
     uint64_t q_full[2], s_full[2][2], p_full[2][2], o_done[2][2];  // [row tile][half]
     uint64_t k_full[kPpStages], k_empty[kPpStages], v_full[kPpStages], v_empty[kPpStages], sc_full[kPpScales];
@@ -347,6 +355,31 @@ __device__ __forceinline__ void pp_store_tile(uint8_t *tile, const uint4 (&raw)[
     }
 }
 
+// The reference for a largest scale (never 0).
+__device__ __forceinline__ float pp_unit(float scale) { return fmaxf(scale / kPpAbove, 0x1p-126f); }
+
+// A tile of a piece whose value scales lie far apart, at position `at` (whole warp): its reference goes to *unit, which
+// has the last one's, and the ratios of the converter warp's two groups are returned.  high: the largest scale of
+// the tiles so far, 0 before the first.
+__device__ __noinline__ float2 pp_follow(const PaParams &p, int b, int head, int at, int len, float *unit, float *high) {
+    const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) - kPpConvWarp0, j = at + lane * 16;
+    float x = 0.0f;
+    if (lane < 8 && j < len) {
+        const int page = p.b.page_table[(long)b * p.b.table_stride + j / p.c.page_size];
+        if (page >= 0 && page < p.c.num_pages) x = p.c.v_scale[(long)page * p.c.kv_heads + head];
+    }
+    const float most = warp_max_butterfly(x), least = -warp_max_butterfly(x > 0.0f ? -x : -INFINITY), was = *high;
+    float vref = *unit;
+    if (most > 0.0f && (was == 0.0f || most > vref * kPpAbove || least < vref * (kPpAbove * kPpExact))) {
+        vref = pp_unit(fmaxf(most, was * kPpDown));
+        __syncwarp();
+        if (lane == 0) *unit = vref, *high = fmaxf(was, most);
+    }
+    __syncwarp();
+    x /= vref;
+    return make_float2(__shfl_sync(0xffffffffu, x, 2 * w), __shfl_sync(0xffffffffu, x, 2 * w + 1));
+}
+
 __device__ void pp_convert(const PaParams &p, PpShared &sm, int u0, int u1) {
     const int lane = threadIdx.x & 31, w = (threadIdx.x >> 5) - kPpConvWarp0;
     int tile = 0;
@@ -373,18 +406,25 @@ __device__ void pp_convert(const PaParams &p, PpShared &sm, int u0, int u1) {
                 }
             }
         };
-        float vref = 0.0f;
+        float high = 0.0f, least = INFINITY;  // of the piece's value scales, zeros aside
+        auto range = [&](float x) { high = fmaxf(high, x), least = fminf(least, x > 0.0f ? x : INFINITY); };
 #pragma unroll 1
         for (int base = (s.n - 1) & ~15; base >= 0; base -= 16) {  // the first sixteen last: they come next
             fetch(base);
-            vref = fmaxf(vref, vs);
+            range(vs);
         }
-        vref = warp_max_butterfly(vref);
+        high = warp_max_butterfly(high), least = -warp_max_butterfly(-least);
         named_sync(2, 128);
-        if (lane == 0) sm.vmax[w] = vref;
+        if (lane == 0) sm.vrange[w] = make_float2(high, least);
         named_sync(2, 128);
-        vref = fmaxf(fmaxf(sm.vmax[0], sm.vmax[1]), fmaxf(sm.vmax[2], sm.vmax[3]));
-        if (!(vref > 0.0f)) vref = 1.0f;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) high = fmaxf(high, sm.vrange[x].x), least = fminf(least, sm.vrange[x].y);
+        // one reference for the piece, or, where that would cost values, the tiles' own
+        high = high > 0.0f ? high : kPpAbove;
+        __syncwarp();
+        if (lane == 0) sm.high[w] = least < high * kPpExact ? 0.0f : -1.0f, sm.unit[w] = pp_unit(high);
+        __syncwarp();
+        vs /= sm.unit[w];  // from here on the ratio
         uint4 kr[8], vr[8];
         // this thread's rows and columns in its two 16-position groups of tile i
         long at[2];
@@ -416,10 +456,11 @@ __device__ void pp_convert(const PaParams &p, PpShared &sm, int u0, int u1) {
             const int st = tile % kPpStages, use = tile / kPpStages;
             PpScale &sc = sm.sc[tile % kPpScales];
             if ((lane >> 1) == (i & 15)) sc.k[2 * w + (lane & 1)] = ks;
-            const float ratio = vs / vref;
-            const __half2 rel[2] = {__float2half2_rn(__shfl_sync(0xffffffffu, ratio, (i & 15) * 2)),
-                                    __float2half2_rn(__shfl_sync(0xffffffffu, ratio, (i & 15) * 2 + 1))};
-            if (w == 0 && lane == 0) sc.vref = vref;
+            float2 r = make_float2(__shfl_sync(0xffffffffu, vs, (i & 15) * 2), __shfl_sync(0xffffffffu, vs, (i & 15) * 2 + 1));
+            if (sm.high[w] >= 0.0f)
+                r = pp_follow(p, s.b, s.h, s.span.step(s.off + i) * kPpKeys, s.seq.len, &sm.unit[w], &sm.high[w]);
+            const __half2 rel[2] = {__float2half2_rn(r.x), __float2half2_rn(r.y)};
+            if (w == 0 && lane == 0) sc.vref = sm.unit[0];
             __syncwarp();
             if (lane == 0) mbar_arrive(&sm.sc_full[tile % kPpScales]);
             if (!(ok = pp_wait_warp(&sm.k_empty[st], (use & 1) ^ 1, sm, p))) break;
@@ -428,7 +469,10 @@ __device__ void pp_convert(const PaParams &p, PpShared &sm, int u0, int u1) {
             __syncwarp();
             if (lane == 0) mbar_arrive(&sm.k_full[st]);
             if (i + 1 < s.n) {
-                if (((i + 1) & 15) == 0) fetch(i + 1);
+                if (((i + 1) & 15) == 0) {
+                    fetch(i + 1);
+                    vs /= sm.unit[w];  // (of no use where the tiles have their own)
+                }
                 place(i + 1);
                 load(p.c.k, kr);
             }
@@ -646,7 +690,8 @@ __device__ void pp_softmax(const PaParams &p, PpShared &sm, int u0, int u1, int 
                     pp_ld32(tsh, v[0]);
                     pp_ld32(tsh + 32, v[1]);
                     float4 ks = *reinterpret_cast<const float4 *>(sc.k + 4 * h);
-                    vref = sc.vref;
+                    const float unit = sc.vref;
+                    if (y == 0) vref = unit;
                     const int key0 = s.span.step(s.off + j) * kPpKeys + 64 * h;
                     const bool whole = key0 + 63 <= pos &&
                                        (p.window <= 0 || pos - key0 < p.window || key0 + 64 <= p.sinks) &
@@ -678,13 +723,14 @@ __device__ void pp_softmax(const PaParams &p, PpShared &sm, int u0, int u1, int 
                         top = fmaxf(top, fmaxf(mx, my) * col[g]);
                     }
                     if (m == -INFINITY) m = top;  // (O and l are zero: there is nothing to scale)
-                    if (__any_sync(0xffffffffu, top > m + kPpLazy)) {
+                    if (__any_sync(0xffffffffu, top > m + kPpLazy || unit != vref)) {
                         const float now = fmaxf(m, top), f = now == -INFINITY ? 1.0f : pa_exp2(m - now);
                         m = now;
                         l *= f;
                         if (!(ok = pp_wait_warp(&sm.o_done[i][h ^ 1], (uint32_t)(used + ((y - 1) >> 1)) & 1, sm, p))) break;
                         tc_fence_after();
-                        pp_scale_o(to, f);
+                        pp_scale_o(to, f * fminf(vref / unit, 0x1p100f));  // (more than 1 / kPpDown only while O is zero)
+                        vref = unit;
                     }
                     const float base = m == -INFINITY ? 0.0f : m;
                     const uint64_t less = pp_pair(-base, -base);
@@ -899,15 +945,17 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_attend_prompt_kernel(cons
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    // launched with 128 registers a thread: 256 x 152 + 128 x 128 + 128 x 80 = 512 x 128
+    // launched with 128 registers a thread: 256 x 144 + 128 x 136 + 128 x 88 = 512 x 128 (an increase waits for the last
+    // group's decrease; a decrease may not name more than the launch gave).  With 152 / 128 / 80 the f16 kernel spills
+    // as well and windowed prompts take 165 us instead of 160, a prompt of 4096 at 16384 1460 instead of 1451.
     if (warp < kPpConvWarp0) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
         pp_softmax<T>(p, sm, u0, u1, share);
     } else if (warp < kPpMmaWarp) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 128;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
         pp_convert(p, sm, u0, u1);
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         if (warp < kPpMmaWarp + 2) pp_products(p, sm, u0, u1);
     }
     tc_fence_before();

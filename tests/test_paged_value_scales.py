@@ -71,3 +71,40 @@ def test_zero_scales_between(pkg, dev):
         c.vs[c.table[b, 2].long()] = 0.0
         c.vs[c.table[b, 5].long()] = 0.0
     check_fine(pkg, dev, c, queries(c, 12, torch.float16))
+
+
+PROMPTS = [(6, 2, [(300, 9000)] * 4), (1, 2, [(257, 5000), (60, 4000)] * 3), (8, 1, [(2000, 2100)]), (6, 2, [(130, 130), (9, 700)])]
+
+
+@pytest.mark.parametrize("page", [16, 64, 128])
+@pytest.mark.parametrize("drop", [16, 24, 40, 80])
+@pytest.mark.parametrize("group,kv,seqs", PROMPTS)
+def test_prompts(pkg, dev, group, kv, seqs, drop, page):
+    """Every third run of 128 positions is large."""
+    c = far_apart(seqs, page, kv, drop, lambda at: at * page // 128 % 3 == 1, seed=drop + page)
+    check_fine(pkg, dev, c, queries(c, kv * group, torch.bfloat16))
+
+
+@pytest.mark.parametrize("page", [16, 32])
+@pytest.mark.parametrize("drop", [14, 20])
+@pytest.mark.parametrize("group,kv,seqs", PROMPTS)
+def test_prompts_within_128_positions(pkg, dev, group, kv, seqs, drop, page):
+    c = far_apart(seqs, page, kv, drop, lambda at: at % 3 == 1, seed=drop + page)
+    check_fine(pkg, dev, c, queries(c, kv * group, torch.bfloat16))
+
+
+@pytest.mark.parametrize("drop", [30, 60])
+def test_prompt_rows_that_do_not_see_the_large_values(pkg, dev, drop):
+    """The last 128 positions are large and only the last rows see them; then the first 128, behind a window."""
+    c = far_apart([(300, 1280), (700, 900)], 64, 2, drop, lambda at: at in (18, 19), seed=drop)
+    check_fine(pkg, dev, c, queries(c, 12, torch.bfloat16, away=False))
+    c = far_apart([(500, 500), (120, 250)], 64, 2, drop, lambda at: at < 2, seed=drop)
+    check_fine(pkg, dev, c, queries(c, 12, torch.bfloat16, away=False), window=40)
+
+
+def test_prompts_with_zero_scales_between(pkg, dev):
+    c = far_apart([(300, 3000), (100, 1500)], 64, 2, 40, lambda at: at // 2 % 3 == 1, seed=4)
+    for b in range(2):
+        for at in (0, 1, 4, 9):
+            c.vs[c.table[b, at].long()] = 0.0
+    check_fine(pkg, dev, c, queries(c, 12, torch.float16))
