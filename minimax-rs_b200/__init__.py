@@ -475,7 +475,7 @@ def _tokens(t, heads, what: str):
         return 0, h, h * HEAD_DIM
     if d != HEAD_DIM or one != 1 or h != (heads or h) or h < 1 or (head != HEAD_DIM and h > 1):
         raise MoeError(MMRS_ERR_ARG, f"{what}: [tokens][{heads or 'heads'}][{HEAD_DIM}], heads side by side")
-    return n, h, row if n > 1 else max(row, h * HEAD_DIM)
+    return n, h, row if n > 1 else h * HEAD_DIM  # (the stride of a single row is never used and may be anything)
 
 
 def _on_gpu(dev: int):
