@@ -454,6 +454,13 @@ def _on_stream(stream):
     return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
 
 
+def _made(t) -> None:
+    """Waits until what a constructor wrote is in place: the first call may run on any stream."""
+    if t.is_cuda:
+        import torch
+        torch.cuda.current_stream(t.device).synchronize()
+
+
 def _same_device(dev: int, *tensors) -> None:
     """The kernels follow raw pointers: every tensor of a call lies on one GPU."""
     if dev < 0:
@@ -528,6 +535,7 @@ class PagedKvCache:
         shape = (num_pages, kv_heads, page_size, HEAD_DIM)
         self._bind(*(torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn) for _ in range(2)),
                    *(torch.zeros(shape[:2], dtype=torch.float32, device=device) for _ in range(2)))
+        _made(self.k)
 
     @classmethod
     def from_tensors(cls, k, v, k_scale, v_scale) -> "PagedKvCache":
@@ -674,6 +682,7 @@ class DraftVerifier:
         self.tokens = torch.full((max_seqs, max_q), -1, dtype=torch.int32, device=device)
         self.accepted = torch.zeros(max_seqs, dtype=torch.int32, device=device)
         self.logprobs = torch.zeros(max_seqs, max_q, dtype=torch.float32, device=device)
+        _made(self.ws)
         self._ptrs = (self.tokens.data_ptr(), self.accepted.data_ptr(), self.logprobs.data_ptr(), self.ws.data_ptr(), need)
 
     def status(self) -> int:
