@@ -12,8 +12,8 @@ namespace mmrs {
 constexpr int kPaMaxSeqs = MMRS_PAGED_MAX_SEQS;
 constexpr int kPaDecodeRows = 32;  // rows of an item of the decode kernel, at most
 // Rows of a KV head up to which a sequence is the decode kernel's: 64 sequences (300000 positions, 8
-// heads) take it 250 us with 30 rows, 369 with 48, 480 with 54, 723 with 96, and the prompt kernel 340 to
-// 350 with any number up to 128; 4 sequences 38 us with 48 rows, 46 with 54, 60 with 96, and 50 to 55.
+// heads) take it 242 us with 30 rows, 362 with 48, 462 with 54, 695 with 96, and the prompt kernel 313 to
+// 330 with any number from 30 to 96; 4 sequences 32 us with 30 rows, 36 with 48, 44 with 54, 58 with 96, and 45 to 51.
 constexpr int kPaFewRows = 48;
 constexpr float kPaLog2e = 1.4426950408889634f;
 constexpr float kPaLn2 = 0.6931471805599453f;

@@ -145,8 +145,9 @@ struct PdKernel {
             f[4 * i] = v.x, f[4 * i + 1] = v.y, f[4 * i + 2] = v.z, f[4 * i + 3] = v.w;
         }
     }
-    // bf16 queries become f16 with the row's largest value moved to [2^14, 2^15): exact but for
-    // values 2^-38 of it and less.  Returns what the products have to be multiplied by.
+    // bf16 queries become f16 with the row's largest value moved to [2^14, 2^15): exact down to 2^-31 of it
+    // (f16's subnormals round eight bits from there on), 0 below 2^-39.  Returns what the products have to be
+    // multiplied by.
     static __device__ float to_f16(uint32_t (&f)[16]) {
         if constexpr (sizeof(T) == 2 && !__is_same(T, __half)) {
             float amax = 0.0f;

@@ -608,8 +608,8 @@ __device__ __forceinline__ float pp_load_q(const PaParams &p, const PpSeg &s, in
     for (int g = 0; g < 4; ++g) {
         uint32_t *w = reinterpret_cast<uint32_t *>(f[g]);
         if constexpr (!__is_same(T, __half)) {
-            // to f16 with the row's largest value moved to [2^14, 2^15): exact but for values 2^-38 of it
-            // and less
+            // to f16 with the row's largest value moved to [2^14, 2^15): exact down to 2^-31 of it (f16's
+            // subnormals round eight bits from there on), 0 below 2^-39
             float amax = 0.0f;
 #pragma unroll
             for (int i = 0; i < 16; ++i)

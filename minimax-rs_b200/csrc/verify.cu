@@ -11,8 +11,9 @@
 //                         the sequence's last block to finish joins the chunks' winners.  It starts
 //                         while the first kernel drains, with its noise on the way.
 // A block reads 64 bytes a thread at once and keeps them in registers: 8192 f32 or 16384 16-bit tokens
-// (8192 of 16 bits: 33 ragged sequences 39 us instead of 37, 320 rows of f16 86 instead of 76).  A row is cut
-// into the number of chunks whose rounds of resident blocks are the shortest.
+// (8192 of 16 bits: 33 ragged sequences 39 us instead of 37, 320 rows of f16 86 instead of 80; that the largest
+// of 16-bit logits is found two at a time makes that 76).  A row is cut into the number of chunks whose rounds of
+// resident blocks are the shortest.
 // Measured (200064 tokens, with the draft model's probabilities unless said): 5 rows of f32 12.8 us in a
 // captured graph (two launches and their dependent reads; the bytes alone would take 0.9); 320 rows of
 // 64 sequences 74 us (362 MB, 4.9 TB/s, 0.74 of a plain copy's); 33 sequences of 1 to 8 bf16 rows without
