@@ -21,7 +21,7 @@
 // relative to a reference, multiplies the values on their way to f16 (exact for the powers of two that the
 // append writes, one rounding otherwise).  Neither costs the softmax anything an element.  The reference is the
 // piece's, from its largest scale; where scales lie more than 2^22 apart, it is each tile's, and O is rescaled
-// with it as with the maximum.  (One reference for the piece and nothing else took 1427 us instead of 1451 at the
+// with it as with the maximum.  (One reference for the piece and nothing else took 1430 us instead of 1447 at the
 // prompt below, and lost the values of pages 2^26 below the largest.)  The running maximum moves only when it
 // grows by more than 2^8 (P stays below f16's range), which leaves O alone on almost every tile.
 //
@@ -33,7 +33,7 @@
 // per SM) takes an equal contiguous part; an item cut by that gets its pieces joined through the
 // workspace by the CTA that finishes last, in order.
 //
-// Measured: 4096 tokens behind 12288 others, 48 + 8 heads, f16: 1451 us from a cold start (994 TFLOP/s,
+// Measured: 4096 tokens behind 12288 others, 48 + 8 heads, f16: 1447 us from a cold start (997 TFLOP/s,
 // 0.61 of what the library's largest product reaches), some 1690 us under the power limit.  The tensor
 // cores are busy 40 % of the time and the exponential units 45 %: what is left is the chain of one
 // half, scores -> maximum -> exponentials -> P -> product, some 2500 cycles with two tiles to fill it
@@ -691,7 +691,6 @@ __device__ void pp_softmax(const PaParams &p, PpShared &sm, int u0, int u1, int 
                     pp_ld32(tsh + 32, v[1]);
                     float4 ks = *reinterpret_cast<const float4 *>(sc.k + 4 * h);
                     const float unit = sc.vref;
-                    if (y == 0) vref = unit;
                     const int key0 = s.span.step(s.off + j) * kPpKeys + 64 * h;
                     const bool whole = key0 + 63 <= pos &&
                                        (p.window <= 0 || pos - key0 < p.window || key0 + 64 <= p.sinks) &
@@ -722,7 +721,7 @@ __device__ void pp_softmax(const PaParams &p, PpShared &sm, int u0, int u1, int 
                         for (int c = 1; c < 8; ++c) mx = fmaxf(mx, x[c]), my = fmaxf(my, x[8 + c]);
                         top = fmaxf(top, fmaxf(mx, my) * col[g]);
                     }
-                    if (m == -INFINITY) m = top;  // (O and l are zero: there is nothing to scale)
+                    if (m == -INFINITY) m = top, vref = unit;  // (O and l are zero: there is nothing to scale)
                     if (__any_sync(0xffffffffu, top > m + kPpLazy || unit != vref)) {
                         const float now = fmaxf(m, top), f = now == -INFINITY ? 1.0f : pa_exp2(m - now);
                         m = now;
@@ -947,7 +946,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) paged_attend_prompt_kernel(cons
     tc_fence_after();
     // launched with 128 registers a thread: 256 x 144 + 128 x 136 + 128 x 88 = 512 x 128 (an increase waits for the last
     // group's decrease; a decrease may not name more than the launch gave).  With 152 / 128 / 80 the f16 kernel spills
-    // as well and windowed prompts take 165 us instead of 160, a prompt of 4096 at 16384 1460 instead of 1451.
+    // as well and windowed prompts take 165 us instead of 160, a prompt of 4096 at 16384 1460 instead of 1447.
     if (warp < kPpConvWarp0) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
         pp_softmax<T>(p, sm, u0, u1, share);
