@@ -41,3 +41,13 @@ def test_long(pkg, dev, seqs, page, size, dtype):
 def test_shapes(pkg, dev, seqs, group, kv, window, sinks):
     c = Case(seqs, 32, kv, seed=group + window)
     check_fine(pkg, dev, c, (c.randn(c.tokens, group * kv, D) * 0.7).half(), window=window, sinks=sinks)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group,kv", [(6, 2), (1, 2), (16, 1)])
+@pytest.mark.parametrize("seqs", [[(5, 3), (1, 0), (2, 900), (8, 8)], [(60, 7), (300, 200), (3, 1)], [(1, 0)], [(70, 0)]])
+def test_more_new_tokens_than_positions(pkg, dev, seqs, group, kv):
+    """Rows before a sequence's first position see nothing: 0 and -infinity, next to rows that do."""
+    c = Case(seqs, 16, kv, seed=group)
+    c.max_len = max(c.max_len, 1)
+    check_fine(pkg, dev, c, (c.randn(c.tokens, group * kv, D) * 0.7).half())
